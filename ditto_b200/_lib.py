@@ -32,6 +32,42 @@ EPILOGUE_QUAD_MMA = 0x400
 EPILOGUE_WIDE_MMA = 0x800
 EPILOGUE_FLOW_MMA = 0x1000
 
+STATUS_BAD_PAGE = 0x10001    # values of the status word beside those of expired waits
+STATUS_NO_PAGES = 0x10002
+
+Strides2, Strides3 = ctypes.c_longlong * 2, ctypes.c_longlong * 3
+
+
+def _block(name, text):
+    """A C struct of the header: "type: names" lines."""
+    types = {"ptr": ctypes.c_void_p, "int": ctypes.c_int, "float": ctypes.c_float, "ll": ctypes.c_longlong, "s2": Strides2, "s3": Strides3}
+    fields = [(f, types[kind]) for line in text.strip().splitlines() for kind, names in [line.split(":")] for f in names.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+MaskedArgs = _block("MaskedArgs", """
+ptr: q k v out lse
+s3: q_strides k_strides v_strides out_strides
+int: batch M L heads kv_heads head_dim dtype causal
+float: scale cap
+ptr: slopes prefix documents""")
+PagedArgs = _block("PagedArgs", """
+ptr: q key_pages value_pages out
+s2: q_strides out_strides
+s3: key_strides value_strides
+ptr: table lengths starts
+ll: table_stride
+int: tokens batch pages page table_cols heads kv_heads head_dim dtype
+float: scale cap
+ptr: slopes prefix""")
+AppendArgs = _block("AppendArgs", """
+ptr: keys values key_pages value_pages
+s2: k_strides v_strides
+s3: key_strides value_strides
+ptr: table lengths starts
+ll: table_stride
+int: tokens batch pages page table_cols kv_heads head_dim""")
+
 EXPORTS = (
     "ditto_b200_bmm_softmax_bmm",
     "ditto_b200_gemm_relu_gemm",
@@ -42,6 +78,11 @@ EXPORTS = (
     "ditto_b200_workspace_bytes",
     "ditto_b200_mlp_cluster_slots",
     "ditto_b200_mlp_tiles_cut",
+    "ditto_b200_masked_workspace_bytes",
+    "ditto_b200_masked_attention",
+    "ditto_b200_paged_workspace_bytes",
+    "ditto_b200_paged_attention",
+    "ditto_b200_cache_append",
     "ditto_b200_selftest_umma",
     "ditto_b200_selftest_umma_pair",
     "ditto_b200_selftest_ex2",
@@ -102,6 +143,16 @@ def load():
     lib.ditto_b200_mlp_cluster_slots.restype = i
     lib.ditto_b200_mlp_tiles_cut.argtypes = [i, i, i, i, i, i, ctypes.POINTER(i)]
     lib.ditto_b200_mlp_tiles_cut.restype = i
+    lib.ditto_b200_masked_workspace_bytes.argtypes = [vp, i]
+    lib.ditto_b200_masked_workspace_bytes.restype = sz
+    lib.ditto_b200_masked_attention.argtypes = [vp, vp, sz, vp, vp]
+    lib.ditto_b200_masked_attention.restype = i
+    lib.ditto_b200_paged_workspace_bytes.argtypes = [vp]
+    lib.ditto_b200_paged_workspace_bytes.restype = sz
+    lib.ditto_b200_paged_attention.argtypes = [vp, vp, sz, vp, vp]
+    lib.ditto_b200_paged_attention.restype = i
+    lib.ditto_b200_cache_append.argtypes = [vp, vp, vp]
+    lib.ditto_b200_cache_append.restype = i
     lib.ditto_b200_selftest_umma.argtypes = [vp, vp, vp, i, i, i, i, i, vp, vp]
     lib.ditto_b200_selftest_umma.restype = i
     lib.ditto_b200_selftest_umma_pair.argtypes = [vp, vp, vp, i, i, i, i, vp, vp]

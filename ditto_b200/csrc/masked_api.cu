@@ -1,0 +1,295 @@
+// C ABI of the masked attention operators and the paged cache: argument checking, tensor maps, scratch memory, launches.
+#include <cmath>
+#include <cstring>
+
+#include "../../include/ditto_b200.h"
+#include "cache_sm100.cuh"
+#include "host_util.cuh"
+#include "masked_plan_sm100.cuh"
+
+namespace {
+
+using namespace ditto_b200;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// strides of a [.., .., .., head_dim] operand in elements: whole 16-byte pieces
+bool strides_ok(const long long* s, int n) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] <= 0 || s[i] % 8 || s[i] >= (1ll << 38)) return false;
+  return true;
+}
+
+int map_4d(CUtensorMap* map, bool bf16, const void* base, uint64_t d, uint64_t n1, uint64_t n2, uint64_t n3, long long s1, long long s2,
+           long long s3, uint32_t b1, uint32_t b2) {
+  const uint64_t dims[4] = {d, n1, n2, n3};
+  const uint64_t strides[3] = {static_cast<uint64_t>(s1) * 2, static_cast<uint64_t>(s2) * 2, static_cast<uint64_t>(s3) * 2};
+  const uint32_t box[4] = {64, b1, b2, 1};
+  return make_tensor_map(map, bf16, base, 4, dims, strides, box);
+}
+
+int sm_count(int* sms) {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = current_device_checked(&dev);
+  if (e != cudaSuccess) return cuda_fail("current device", e);
+  int n = known[dev].load(std::memory_order_acquire);
+  if (n == 0) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return cuda_fail("multiprocessor count", e);
+    known[dev].store(n, std::memory_order_release);
+  }
+  *sms = n;
+  return DITTO_OK;
+}
+
+// What the score rules of a call make of the kernel's constants.
+int set_rules(masked::Params& p, float scale, float cap, const float* slopes, const int* prefix, int causal) {
+  if (!(scale > 0.f) || !std::isfinite(scale) || !(cap >= 0.f) || !std::isfinite(cap)) return DITTO_ERR_INVALID_ARG;
+  if (causal != 0 && causal != 1) return DITTO_ERR_INVALID_ARG;
+  if (prefix != nullptr && !causal) return DITTO_ERR_INVALID_ARG;
+  p.causal = causal;
+  p.slopes = slopes;
+  p.prefix = prefix;
+  p.score_log2 = scale * kLog2e;
+  p.cap_in = cap > 0.f ? 2.0f * scale * kLog2e / cap : 0.f;
+  p.cap_out = cap > 0.f ? cap * kLog2e : 0.f;
+  p.c = cap > 0.f || slopes != nullptr ? 1.0f : p.score_log2;
+  return DITTO_OK;
+}
+
+int check_heads(int heads, int kv_heads, int d, int dtype) {
+  if (heads <= 0 || kv_heads <= 0 || d <= 0) return DITTO_ERR_INVALID_ARG;
+  if (dtype != DITTO_DTYPE_FP16 && dtype != DITTO_DTYPE_BF16) return DITTO_ERR_UNSUPPORTED;
+  if (heads % kv_heads || heads / kv_heads > 128 || d % 8 || d > 128) return DITTO_ERR_UNSUPPORTED;
+  return DITTO_OK;
+}
+
+int check_masked(const ditto_b200_masked_args* a) {
+  if (!a || !a->q || !a->k || !a->v || !a->out) return DITTO_ERR_INVALID_ARG;
+  if (a->batch <= 0 || a->M <= 0 || a->L <= 0) return DITTO_ERR_INVALID_ARG;
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) return DITTO_ERR_INVALID_ARG;
+  if (!strides_ok(a->q_strides, 3) || !strides_ok(a->k_strides, 3) || !strides_ok(a->v_strides, 3) || !strides_ok(a->out_strides, 3))
+    return DITTO_ERR_INVALID_ARG;
+  if (a->documents != nullptr && a->M > a->L) return DITTO_ERR_INVALID_ARG;
+  return check_heads(a->heads, a->kv_heads, a->head_dim, a->dtype);
+}
+
+struct MaskedScratch {
+  size_t key_blocks, hulls, key_hulls, bytes;
+};
+MaskedScratch masked_scratch(const ditto_b200_masked_args* a, bool backward) {
+  MaskedScratch s = {};
+  if (a->documents != nullptr) {
+    const size_t blocks = (a->L + 127) / 128, tile_tokens = 128 / (a->heads / a->kv_heads), tiles = (a->M + tile_tokens - 1) / tile_tokens;
+    s.hulls = up256(a->batch * blocks * sizeof(masked::KeyBlock));
+    s.key_hulls = s.hulls + up256(a->batch * tiles * sizeof(int2));
+    s.bytes = s.key_hulls + (backward ? up256(a->batch * blocks * sizeof(int2)) : 0);
+  }
+  return s;
+}
+
+// Query tiles of an item: two where that still leaves an item for every SM, so that each block of keys is loaded once for both.
+int tiles_of_item(long long tiles, long long heads, int sms) { return tiles >= 2 && heads * ((tiles + 1) / 2) >= sms ? 2 : 1; }
+
+int fill_masked(masked::Params& p, const ditto_b200_masked_args* a) {
+  std::memset(&p, 0, sizeof(p));
+  int rc = set_rules(p, a->scale, a->cap, a->slopes, a->prefix, a->causal);
+  if (rc) return rc;
+  const bool bf16 = a->dtype == DITTO_DTYPE_BF16;
+  p.batch = a->batch;
+  p.M = a->M;
+  p.L = a->L;
+  p.heads = a->heads;
+  p.kv_heads = a->kv_heads;
+  p.group = a->heads / a->kv_heads;
+  p.tile_tokens = 128 / p.group;
+  p.tiles = (a->M + p.tile_tokens - 1) / p.tile_tokens;
+  p.d = a->head_dim;
+  p.documents = a->documents;
+  p.out = a->out;
+  p.lse = a->lse;
+  p.out_batch = a->out_strides[0];
+  p.out_token = a->out_strides[1];
+  p.out_head = a->out_strides[2];
+  rc = map_4d(&p.map_q, bf16, a->q, p.d, p.heads, p.M, p.batch, a->q_strides[2], a->q_strides[1], a->q_strides[0], p.group, p.tile_tokens);
+  if (rc) return rc;
+  rc = map_4d(&p.map_k, bf16, a->k, p.d, p.L, p.kv_heads, p.batch, a->k_strides[1], a->k_strides[2], a->k_strides[0], 128, 1);
+  if (rc) return rc;
+  return map_4d(&p.map_v, bf16, a->v, p.d, p.L, p.kv_heads, p.batch, a->v_strides[1], a->v_strides[2], a->v_strides[0], 128, 1);
+}
+
+// The CTAs of a paged call and the query tiles of its items.
+struct PagedPlan {
+  int grid, tiles;
+  size_t part_ml, parts, bytes;
+};
+int paged_plan(const ditto_b200_paged_args* a, PagedPlan* plan) {
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc) return rc;
+  const int group = a->heads / a->kv_heads, tile_tokens = 128 / group, d = a->head_dim <= 64 ? 64 : 128;
+  // as many tiles as the sequences have on average: a second tile an item only where most sequences fill one
+  plan->tiles = a->starts != nullptr && static_cast<long long>(a->tokens) > static_cast<long long>(a->batch) * tile_tokens ? 2 : 1;
+  const long long items = (a->starts != nullptr ? a->tokens / (tile_tokens * plan->tiles) + static_cast<long long>(a->batch) : a->batch) * a->kv_heads;
+  const long long most = items * ((static_cast<long long>(a->table_cols) * a->page + 127) / 128);
+  plan->grid = static_cast<int>(most < sms ? most : sms);
+  const size_t rows = static_cast<size_t>(plan->grid) * 2 * plan->tiles * 128;
+  plan->part_ml = up256(rows * d * sizeof(float));
+  plan->parts = plan->part_ml + up256(rows * sizeof(float2));
+  plan->bytes = plan->parts + up256(plan->grid * sizeof(masked::PartDesc));
+  return DITTO_OK;
+}
+
+int check_paged(const ditto_b200_paged_args* a) {
+  if (!a || !a->q || !a->key_pages || !a->value_pages || !a->out || !a->table || !a->lengths) return DITTO_ERR_INVALID_ARG;
+  if (a->tokens <= 0 || a->batch <= 0 || a->pages <= 0 || a->page <= 0 || a->table_cols <= 0 || a->table_stride <= 0) return DITTO_ERR_INVALID_ARG;
+  if (a->starts == nullptr && a->tokens != a->batch) return DITTO_ERR_INVALID_ARG;
+  if (!aligned16(a->q) || !aligned16(a->key_pages) || !aligned16(a->value_pages) || !aligned16(a->out)) return DITTO_ERR_INVALID_ARG;
+  if (!strides_ok(a->q_strides, 2) || !strides_ok(a->out_strides, 2) || !strides_ok(a->key_strides, 3) || !strides_ok(a->value_strides, 3))
+    return DITTO_ERR_INVALID_ARG;
+  const bool page_ok = a->page % 128 == 0 || a->page == 16 || a->page == 32 || a->page == 64;
+  if (!page_ok || static_cast<long long>(a->table_cols) * a->page > (1ll << 30)) return DITTO_ERR_UNSUPPORTED;
+  return check_heads(a->heads, a->kv_heads, a->head_dim, a->dtype);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ditto_b200_masked_workspace_bytes(const ditto_b200_masked_args* a, int backward) {
+  if (check_masked(a)) return 0;
+  return masked_scratch(a, backward != 0).bytes;
+}
+
+int ditto_b200_masked_attention(const ditto_b200_masked_args* a, void* workspace, size_t ws_bytes, int* status_word, void* stream) {
+  int rc = check_masked(a);
+  if (rc) return rc;
+  masked::Params p;
+  rc = fill_masked(p, a);
+  if (rc) return rc;
+  const MaskedScratch ws = masked_scratch(a, false);
+  if (ws.bytes > 0 && (workspace == nullptr || ws_bytes < ws.bytes)) return DITTO_ERR_WORKSPACE;
+  if (ws.bytes > 0 && !aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long heads = static_cast<long long>(p.batch) * p.kv_heads;
+  const int nt = tiles_of_item(p.tiles, heads, sms);
+  const long long items = heads * ((p.tiles + nt - 1) / nt);
+  if (items > 0x3fffffffLL) return DITTO_ERR_UNSUPPORTED;
+  p.items = static_cast<int>(items);
+  p.status = status_word;
+  if (a->documents != nullptr) {
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    auto* key_blocks = reinterpret_cast<masked::KeyBlock*>(base);
+    auto* hulls = reinterpret_cast<int2*>(base + ws.hulls);
+    p.key_blocks = key_blocks;
+    p.hulls = hulls;
+    const cudaError_t e = masked::launch_document_plan(a->documents, a->prefix, p.batch, p.M, p.L, p.causal, p.tile_tokens, p.tiles, key_blocks,
+                                                       hulls, nullptr, st);
+    if (e != cudaSuccess) return cuda_fail("masked_attention plan", e);
+  }
+  const cudaError_t e = masked::launch_forward_any(p, p.d <= 64 ? 64 : 128, a->dtype == DITTO_DTYPE_BF16, false, nt,
+                                                   static_cast<int>(items < sms ? items : sms), st);
+  if (e != cudaSuccess) return cuda_fail("masked_attention launch", e);
+  return DITTO_OK;
+}
+
+size_t ditto_b200_paged_workspace_bytes(const ditto_b200_paged_args* a) {
+  PagedPlan plan;
+  if (check_paged(a) || paged_plan(a, &plan)) return 0;
+  return plan.bytes;
+}
+
+int ditto_b200_paged_attention(const ditto_b200_paged_args* a, void* workspace, size_t ws_bytes, int* status_word, void* stream) {
+  int rc = check_paged(a);
+  if (rc) return rc;
+  masked::Params p;
+  std::memset(&p, 0, sizeof(p));
+  rc = set_rules(p, a->scale, a->cap, a->slopes, a->prefix, 1);
+  if (rc) return rc;
+  PagedPlan plan;
+  rc = paged_plan(a, &plan);
+  if (rc) return rc;
+  if (workspace == nullptr || ws_bytes < plan.bytes) return DITTO_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
+  const bool bf16 = a->dtype == DITTO_DTYPE_BF16;
+  const int d = a->head_dim <= 64 ? 64 : 128;
+  p.batch = a->batch;
+  p.M = a->tokens;
+  p.L = a->table_cols * a->page;
+  p.heads = a->heads;
+  p.kv_heads = a->kv_heads;
+  p.group = a->heads / a->kv_heads;
+  p.tile_tokens = 128 / p.group;
+  p.d = a->head_dim;
+  p.out = a->out;
+  p.out_token = a->out_strides[0];
+  p.out_head = a->out_strides[1];
+  p.table = a->table;
+  p.table_stride = a->table_stride;
+  p.lengths = a->lengths;
+  p.starts = a->starts;
+  p.page = a->page;
+  p.pages = a->pages;
+  p.status = status_word;
+  const long long q_all = a->q_strides[0] * static_cast<long long>(a->tokens);
+  rc = map_4d(&p.map_q, bf16, a->q, p.d, p.heads, p.M, 1, a->q_strides[1], a->q_strides[0], q_all, p.group, p.tile_tokens);
+  if (rc) return rc;
+  const uint32_t rows = a->page < 128 ? a->page : 128;
+  rc = map_4d(&p.map_k, bf16, a->key_pages, p.d, p.page, p.kv_heads, p.pages, a->key_strides[1], a->key_strides[2], a->key_strides[0], rows, 1);
+  if (rc) return rc;
+  rc = map_4d(&p.map_v, bf16, a->value_pages, p.d, p.page, p.kv_heads, p.pages, a->value_strides[1], a->value_strides[2], a->value_strides[0], rows, 1);
+  if (rc) return rc;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  p.part_o = reinterpret_cast<float*>(base);
+  p.part_ml = reinterpret_cast<float2*>(base + plan.part_ml);
+  p.parts = reinterpret_cast<masked::PartDesc*>(base + plan.parts);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = masked::launch_forward_any(p, d, bf16, true, plan.tiles, plan.grid, st);
+  if (e == cudaSuccess) e = masked::launch_sum_parts(p, d, bf16, plan.tiles, plan.grid, st);
+  if (e != cudaSuccess) return cuda_fail("paged_attention launch", e);
+  return DITTO_OK;
+}
+
+int ditto_b200_cache_append(const ditto_b200_append_args* a, int* status_word, void* stream) {
+  if (!a || !a->keys || !a->values || !a->key_pages || !a->value_pages || !a->table || !a->lengths) return DITTO_ERR_INVALID_ARG;
+  if (a->tokens <= 0 || a->batch <= 0 || a->pages <= 0 || a->page <= 0 || a->table_cols <= 0 || a->table_stride <= 0 || a->kv_heads <= 0)
+    return DITTO_ERR_INVALID_ARG;
+  if (a->starts == nullptr && a->tokens != a->batch) return DITTO_ERR_INVALID_ARG;
+  if (a->head_dim <= 0 || a->head_dim % 8) return DITTO_ERR_UNSUPPORTED;
+  if (!aligned16(a->keys) || !aligned16(a->values) || !aligned16(a->key_pages) || !aligned16(a->value_pages)) return DITTO_ERR_INVALID_ARG;
+  if (!strides_ok(a->k_strides, 2) || !strides_ok(a->v_strides, 2) || !strides_ok(a->key_strides, 3) || !strides_ok(a->value_strides, 3))
+    return DITTO_ERR_INVALID_ARG;
+  cache::AppendParams p = {};
+  p.keys = static_cast<const uint8_t*>(a->keys);
+  p.values = static_cast<const uint8_t*>(a->values);
+  p.key_pages = static_cast<uint8_t*>(a->key_pages);
+  p.value_pages = static_cast<uint8_t*>(a->value_pages);
+  p.k_token = a->k_strides[0] * 2, p.k_head = a->k_strides[1] * 2;
+  p.v_token = a->v_strides[0] * 2, p.v_head = a->v_strides[1] * 2;
+  p.kp_page = a->key_strides[0] * 2, p.kp_slot = a->key_strides[1] * 2, p.kp_head = a->key_strides[2] * 2;
+  p.vp_page = a->value_strides[0] * 2, p.vp_slot = a->value_strides[1] * 2, p.vp_head = a->value_strides[2] * 2;
+  p.table = a->table;
+  p.table_stride = a->table_stride;
+  p.table_cols = a->table_cols;
+  p.lengths = a->lengths;
+  p.starts = a->starts;
+  p.batch = a->batch;
+  p.tokens = a->tokens;
+  p.kv_heads = a->kv_heads;
+  p.pieces = a->head_dim / 8;
+  p.page = a->page;
+  p.pages = a->pages;
+  p.status = status_word;
+  const cudaError_t e = cache::launch_append(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail("cache_append launch", e);
+  return DITTO_OK;
+}
+
+}  // extern "C"

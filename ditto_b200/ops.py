@@ -391,3 +391,7 @@ def ffn(x, w1, b1, w2, b2, out=None, act1="relu", act2="relu", weight_layout="OI
     _enable_fast(x.device)
     launch_count += 1
     return out
+
+
+# attention with masks and modified scores, and over a paged cache (they use what this module defines)
+from .masked import cache_append, masked_attention, masked_attention_backward, paged_attention  # noqa: E402,F401

@@ -172,6 +172,67 @@ int ditto_b200_mlp_cluster_slots(int dtype, int variant);
  * Needs no GPU.  No counterpart in the reference. */
 int ditto_b200_mlp_tiles_cut(int gemm, int batch, int M, int N, int K, int L, int* cut);
 
+/* Attention with masks and modified scores over dense tensors, with gradients.  No counterpart in the reference, whose chains have
+ * neither.  For query i of head h, at position pos = i + L - M, and key j of its key head h / (heads / kv_heads):
+ *   s = scale q_i . k_j;  cap > 0: s = cap tanh(s / cap);  slopes: s -= slopes[h] |pos - j|
+ *   seen: (not causal, or j <= pos, or j < prefix[b]) and (no documents, or documents[b][pos] == documents[b][j] >= 0)
+ *   out = sum over the seen of softmax(s) v,  lse = log sum exp(s);  a row that sees nothing has out 0 and lse -infinity.
+ * q, out [batch, M, heads, head_dim], k, v [batch, L, kv_heads, head_dim], fp16 or bf16, of any strides that are multiples of eight
+ * elements with contiguous rows of head_dim; lse [batch, M, heads] float32 (may be NULL).
+ * Values where documents are negative may be anything finite; head_dim a multiple of 8 up to 128; heads / kv_heads up to 128; any M, L >= 1
+ * (M <= L with documents). */
+typedef struct {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  long long q_strides[3], k_strides[3], v_strides[3], out_strides[3]; /* batch, token, head; in elements */
+  int batch, M, L, heads, kv_heads, head_dim, dtype, causal;
+  float scale, cap;       /* cap 0: none */
+  const float* slopes;    /* [heads] or NULL */
+  const int* prefix;      /* [batch] or NULL; causal only */
+  const int* documents;   /* [batch, L] or NULL */
+} ditto_b200_masked_args;
+/* Scratch bytes that a call needs (0: none); contents irrelevant on entry, undefined on return. */
+size_t ditto_b200_masked_workspace_bytes(const ditto_b200_masked_args* args, int backward);
+int ditto_b200_masked_attention(const ditto_b200_masked_args* args, void* workspace, size_t ws_bytes, int* status_word, void* stream);
+
+/* Attention of new tokens over a paged cache that holds their keys and values already.  No counterpart in the reference.
+ * Tokens starts[b] .. starts[b + 1] of q (starts NULL: token b) are the last of sequence b's lengths[b] positions; position j of it is slot
+ * j % page of page table[b][j / page].  Scores and masks as above, causal, the same prefix, cap and slopes.
+ * q, out [tokens, heads, head_dim], key_pages, value_pages [pages, page, kv_heads, head_dim], of strides as above.  page 16, 32, 64 or a
+ * multiple of 128.  Slots behind a sequence's end may hold anything, tokens behind the last sequence are left as they are.  A page id out of
+ * range stands for zeros and stores DITTO_STATUS_BAD_PAGE in *status_word; lengths are cut to what a row of the table reaches. */
+#define DITTO_STATUS_BAD_PAGE 0x10001
+#define DITTO_STATUS_NO_PAGES 0x10002
+typedef struct {
+  const void *q, *key_pages, *value_pages;
+  void* out;
+  long long q_strides[2], out_strides[2];       /* token, head; in elements */
+  long long key_strides[3], value_strides[3];   /* page, slot, head */
+  const int *table, *lengths, *starts;          /* [batch, table_cols], [batch], [batch + 1] or NULL */
+  long long table_stride;                       /* entries between rows of the table */
+  int tokens, batch, pages, page, table_cols, heads, kv_heads, head_dim, dtype;
+  float scale, cap;
+  const float* slopes;
+  const int* prefix;
+} ditto_b200_paged_args;
+size_t ditto_b200_paged_workspace_bytes(const ditto_b200_paged_args* args);   /* needed; contents irrelevant on entry */
+int ditto_b200_paged_attention(const ditto_b200_paged_args* args, void* workspace, size_t ws_bytes, int* status_word, void* stream);
+
+/* Writes new tokens' keys and values [tokens, kv_heads, head_dim] to their places in the pages: the places that ditto_b200_paged_attention
+ * with the same table, lengths and starts reads them from.  16-bit elements of either type.  Places without a valid page are passed over
+ * and store DITTO_STATUS_BAD_PAGE. */
+typedef struct {
+  const void *keys, *values;
+  void *key_pages, *value_pages;
+  long long k_strides[2], v_strides[2];
+  long long key_strides[3], value_strides[3];
+  const int *table, *lengths, *starts;
+  long long table_stride;
+  int tokens, batch, pages, page, table_cols, kv_heads, head_dim;
+} ditto_b200_append_args;
+int ditto_b200_cache_append(const ditto_b200_append_args* args, int* status_word, void* stream);
+
 /* Single-CTA check of one tcgen05 MMA chain: c[128, N] (fp32) = a[128, K] * b.
  *   b_mn 0: b is [N, K]; 1: b is [K, N].  a_tmem 1: the A operand is read from tensor memory.
  * N, K multiples of 64, at most 256.  Exists so the descriptor encodings the fused kernels depend
