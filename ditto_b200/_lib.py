@@ -80,6 +80,7 @@ EXPORTS = (
     "ditto_b200_mlp_tiles_cut",
     "ditto_b200_masked_workspace_bytes",
     "ditto_b200_masked_attention",
+    "ditto_b200_masked_attention_backward",
     "ditto_b200_paged_workspace_bytes",
     "ditto_b200_paged_attention",
     "ditto_b200_cache_append",
@@ -147,6 +148,8 @@ def load():
     lib.ditto_b200_masked_workspace_bytes.restype = sz
     lib.ditto_b200_masked_attention.argtypes = [vp, vp, sz, vp, vp]
     lib.ditto_b200_masked_attention.restype = i
+    lib.ditto_b200_masked_attention_backward.argtypes = [vp, vp, ctypes.POINTER(ctypes.c_longlong), vp, vp, vp, vp, sz, vp, vp]
+    lib.ditto_b200_masked_attention_backward.restype = i
     lib.ditto_b200_paged_workspace_bytes.argtypes = [vp]
     lib.ditto_b200_paged_workspace_bytes.restype = sz
     lib.ditto_b200_paged_attention.argtypes = [vp, vp, sz, vp, vp]

@@ -18,7 +18,7 @@ SOURCES = ["api.cu", "host_util.cu", "attention_sm100.cu", "attention_persistent
            "cache_sm100.cu"]
 # sources that are compiled in parts, an object and a GPU module each: (file, macro, number of parts)
 IN_PARTS = [("mlp_tiles_kernel_sm100.cu", "DITTO_TILES_PART", 8), ("mlp_waves_kernel_sm100.cu", "DITTO_WAVES_PART", 8),
-            ("masked_forward_sm100.cu", "DITTO_MASKED_PART", 8)]
+            ("masked_forward_sm100.cu", "DITTO_MASKED_PART", 8), ("masked_backward_sm100.cu", "DITTO_MASKED_BACKWARD_PART", 4)]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "--use_fast_math",

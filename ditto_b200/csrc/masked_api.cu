@@ -5,6 +5,7 @@
 #include "../../include/ditto_b200.h"
 #include "cache_sm100.cuh"
 #include "host_util.cuh"
+#include "masked_backward_sm100.cuh"
 #include "masked_plan_sm100.cuh"
 
 namespace {
@@ -79,15 +80,24 @@ int check_masked(const ditto_b200_masked_args* a) {
 }
 
 struct MaskedScratch {
-  size_t key_blocks, hulls, key_hulls, bytes;
+  size_t hulls, key_hulls;               // behind the blocks of keys
+  size_t rows, norms, part, parts;       // of the backward pass
+  size_t bytes;
 };
-MaskedScratch masked_scratch(const ditto_b200_masked_args* a, bool backward) {
+MaskedScratch masked_scratch(const ditto_b200_masked_args* a, bool backward, int sms) {
   MaskedScratch s = {};
+  const size_t blocks = (a->L + 127) / 128, tile_tokens = 128 / (a->heads / a->kv_heads), tiles = (a->M + tile_tokens - 1) / tile_tokens;
   if (a->documents != nullptr) {
-    const size_t blocks = (a->L + 127) / 128, tile_tokens = 128 / (a->heads / a->kv_heads), tiles = (a->M + tile_tokens - 1) / tile_tokens;
     s.hulls = up256(a->batch * blocks * sizeof(masked::KeyBlock));
     s.key_hulls = s.hulls + up256(a->batch * tiles * sizeof(int2));
     s.bytes = s.key_hulls + (backward ? up256(a->batch * blocks * sizeof(int2)) : 0);
+  }
+  if (backward) {
+    s.rows = s.bytes;
+    s.norms = s.rows + up256(a->batch * a->kv_heads * tiles * sizeof(masked::TileRows));
+    s.part = s.norms + 256;
+    s.parts = s.part + static_cast<size_t>(sms) * 2 * 2 * 128 * (a->head_dim <= 64 ? 64 : 128) * sizeof(float);
+    s.bytes = s.parts + up256(sms * sizeof(masked::KeyPartDesc));
   }
   return s;
 }
@@ -161,8 +171,9 @@ int check_paged(const ditto_b200_paged_args* a) {
 extern "C" {
 
 size_t ditto_b200_masked_workspace_bytes(const ditto_b200_masked_args* a, int backward) {
-  if (check_masked(a)) return 0;
-  return masked_scratch(a, backward != 0).bytes;
+  int sms = 0;
+  if (check_masked(a) || (backward && sm_count(&sms))) return 0;
+  return masked_scratch(a, backward != 0, sms).bytes;
 }
 
 int ditto_b200_masked_attention(const ditto_b200_masked_args* a, void* workspace, size_t ws_bytes, int* status_word, void* stream) {
@@ -171,7 +182,7 @@ int ditto_b200_masked_attention(const ditto_b200_masked_args* a, void* workspace
   masked::Params p;
   rc = fill_masked(p, a);
   if (rc) return rc;
-  const MaskedScratch ws = masked_scratch(a, false);
+  const MaskedScratch ws = masked_scratch(a, false, 0);
   if (ws.bytes > 0 && (workspace == nullptr || ws_bytes < ws.bytes)) return DITTO_ERR_WORKSPACE;
   if (ws.bytes > 0 && !aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
   int sms = 0;
@@ -197,6 +208,74 @@ int ditto_b200_masked_attention(const ditto_b200_masked_args* a, void* workspace
   const cudaError_t e = masked::launch_forward_any(p, p.d <= 64 ? 64 : 128, a->dtype == DITTO_DTYPE_BF16, false, nt,
                                                    static_cast<int>(items < sms ? items : sms), st);
   if (e != cudaSuccess) return cuda_fail("masked_attention launch", e);
+  return DITTO_OK;
+}
+
+int ditto_b200_masked_attention_backward(const ditto_b200_masked_args* a, const void* grad_out, const long long* grad_strides, void* dq, void* dk,
+                                         void* dv, void* workspace, size_t ws_bytes, int* status_word, void* stream) {
+  int rc = check_masked(a);
+  if (rc) return rc;
+  if (!a->lse || !grad_out || !grad_strides || !dq || !dk || !dv) return DITTO_ERR_INVALID_ARG;
+  if (!aligned16(grad_out) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || !strides_ok(grad_strides, 3)) return DITTO_ERR_INVALID_ARG;
+  masked::Params f;
+  rc = fill_masked(f, a);
+  if (rc) return rc;
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc) return rc;
+  const MaskedScratch ws = masked_scratch(a, true, sms);
+  if (workspace == nullptr || ws_bytes < ws.bytes) return DITTO_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
+  const bool bf16 = a->dtype == DITTO_DTYPE_BF16;
+  masked::BackwardParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.map_q = f.map_q;
+  p.map_k = f.map_k;
+  p.map_v = f.map_v;
+  rc = map_4d(&p.map_do, bf16, grad_out, f.d, f.heads, f.M, f.batch, grad_strides[2], grad_strides[1], grad_strides[0], f.group, f.tile_tokens);
+  if (rc) return rc;
+  p.o = a->out;
+  p.grad = grad_out;
+  p.v = a->v;
+  for (int i = 0; i < 3; ++i) {
+    p.o_stride[i] = a->out_strides[i];
+    p.g_stride[i] = grad_strides[i];
+    p.v_stride[i] = a->v_strides[i];
+  }
+  p.lse = a->lse;
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  p.batch = f.batch, p.M = f.M, p.L = f.L, p.heads = f.heads, p.kv_heads = f.kv_heads, p.group = f.group, p.tile_tokens = f.tile_tokens, p.d = f.d;
+  p.tiles = f.tiles;
+  p.blocks = (f.L + 127) / 128;
+  const long long heads = static_cast<long long>(p.batch) * p.kv_heads;
+  if (heads * p.tiles > 0x3fffffffLL || heads * p.blocks * p.tiles > 0x3fffffffLL) return DITTO_ERR_UNSUPPORTED;
+  p.items = static_cast<int>(heads * p.tiles);
+  p.causal = f.causal, p.c = f.c, p.cap_in = f.cap_in, p.cap_out = f.cap_out, p.score_log2 = f.score_log2, p.scale = a->scale;
+  p.slopes = f.slopes, p.prefix = f.prefix, p.documents = f.documents;
+  p.status = status_word;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  p.rows = reinterpret_cast<masked::TileRows*>(base + ws.rows);
+  p.norms = reinterpret_cast<uint32_t*>(base + ws.norms);
+  p.part = reinterpret_cast<float*>(base + ws.part);
+  p.parts = reinterpret_cast<masked::KeyPartDesc*>(base + ws.parts);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (a->documents != nullptr) {
+    auto* key_blocks = reinterpret_cast<masked::KeyBlock*>(base);
+    auto* hulls = reinterpret_cast<int2*>(base + ws.hulls);
+    auto* key_hulls = reinterpret_cast<int2*>(base + ws.key_hulls);
+    p.key_blocks = key_blocks, p.hulls = hulls, p.key_hulls = key_hulls;
+    e = masked::launch_document_plan(a->documents, a->prefix, p.batch, p.M, p.L, p.causal, p.tile_tokens, p.tiles, key_blocks, hulls, key_hulls, st);
+  }
+  if (e == cudaSuccess) {
+    if (p.d <= 64)
+      e = bf16 ? masked::launch_backward<64, true>(p, sms, st) : masked::launch_backward<64, false>(p, sms, st);
+    else
+      e = bf16 ? masked::launch_backward<128, true>(p, sms, st) : masked::launch_backward<128, false>(p, sms, st);
+  }
+  if (e != cudaSuccess) return cuda_fail("masked_attention_backward launch", e);
   return DITTO_OK;
 }
 

@@ -1,0 +1,973 @@
+// Gradients of masked attention, from P = 2^(c s - lse):  dV = P^T dO,  dS = P (dO V^T - delta) (1 - tanh^2),  dQ = scale dS K,
+// dK = scale dS^T Q,  delta_i = sum_d dO_id O_id.
+//
+// Three launches: delta with the other things the kernels need of a query row, in tile order; the keys' gradients; the queries'.  The last
+// two compute the scores and dO V^T each for themselves (seven products instead of five), so that every sum stays in tensor memory in one
+// CTA, in a fixed order: no atomics, no accumulator that passes through memory for every block.
+//
+// Keys: a block of 128 keys stays, the query tiles pass.  S^T = K Q^T and dP^T = V dO^T have keys as rows, so that P^T and dS^T go back to
+// tensor memory as the first operands of dV += P^T dO and dK += dS^T Q without a transposition.  Two MMA warps: (dV, next S^T) runs under
+// the second half of a tile's arithmetic and (dK, next dP^T) under the first half of the next tile's.  The tiles of all blocks are dealt
+// out in equal shares to the CTAs (causal masks make blocks unequal, shared key heads make them few and long); blocks that a share cuts are
+// summed from fp32 parts, in order.
+// Queries: a tile stays, the blocks of keys pass; dS goes over dP, of which there are two so that the next one is ready early.
+//
+// fp16: P is taken times 2^14 and dS times a power of two from the largest row norms of dO and V, so that neither leaves the type's range
+// nor falls below its normal numbers as weights of a few thousand keys would.
+#include <atomic>
+
+#include "host_util.cuh"
+#include "masked_backward_sm100.cuh"
+#include "mlp_common.cuh"
+#include "sm100_ptx.cuh"
+#include "softmax_step.cuh"
+
+#ifndef DITTO_MASKED_BACKWARD_PART
+#define DITTO_MASKED_BACKWARD_PART 0
+#endif
+
+namespace ditto_b200 {
+namespace masked {
+namespace {
+
+constexpr int kComputeWarps = 8, kThreads = 32 * (kComputeWarps + 3);
+constexpr int kProducerWarp = kComputeWarps, kMmaWarp = kComputeWarps + 1;      // (two MMA warps)
+constexpr uint32_t kTmemCols = 512, kColS = 0, kColDp = 128, kColAcc = 256;
+constexpr int kSegs = 4;
+constexpr float kPScaleLog2 = 14.0f;                   // of P in fp16
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// 2^k and 2^-k for dS in fp16: |dS| <= |dO_i| (|V_j| + |O_i|) <= 2 max |dO| max |V|, which 2^k takes to at most 2^15.
+template <bool BF16>
+__device__ __forceinline__ void ds_scale(const BackwardParams& p, float* up, float* down) {
+  *up = *down = 1.0f;
+  if constexpr (!BF16) {
+    const float a = __uint_as_float(p.norms[0]), b = __uint_as_float(p.norms[1]);      // squares
+    const float bound = sqrtf(a) * sqrtf(b);
+    if (bound > 0.f && bound < INFINITY) {
+      const int e = min(100, max(-100, 14 - (static_cast<int>(__float_as_uint(bound) >> 23) - 127 + 1)));
+      *up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      *down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ rows
+constexpr int kRowThreads = 256;
+
+template <bool BF16>
+__device__ __forceinline__ void dot8(uint4 a, uint4 b, float& dot, float& norm_a) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = unpack2<BF16>(x[i]), v = unpack2<BF16>(y[i]);
+    dot = fmaf(u.x, v.x, fmaf(u.y, v.y, dot));
+    norm_a = fmaf(u.x, u.x, fmaf(u.y, u.y, norm_a));
+  }
+}
+
+// Half a warp a row.  Bound by reading out and its gradient once.
+template <bool BF16>
+__global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid_constant__ BackwardParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 15, pieces = p.d / 8;
+  const long long rows = static_cast<long long>(p.batch) * p.kv_heads * p.tiles * kRows, step = static_cast<long long>(gridDim.x) * (kRowThreads / 16);
+  float norm_g = 0.f, norm_v = 0.f;
+  // (the loops' bounds are those of whole warps: shuffles)
+  for (long long at = static_cast<long long>(blockIdx.x) * (kRowThreads / 16) + threadIdx.x / 16; at - (threadIdx.x / 16 & 1) < rows; at += step) {
+    const int r = static_cast<int>(at % kRows);
+    long long rest = at / kRows;
+    const int tile = static_cast<int>(rest % p.tiles);
+    rest /= p.tiles;
+    const int kv_head = static_cast<int>(rest % p.kv_heads), b = static_cast<int>(rest / p.kv_heads);
+    const int token = tile * p.tile_tokens + r / p.group, head = kv_head * p.group + r % p.group, pos = token + p.L - p.M;
+    const bool valid = at < rows && r / p.group < p.tile_tokens && token < p.M;
+    float dot = 0.f, norm = 0.f;
+    if (valid && lane < pieces) {
+      const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.grad) + 2 * (b * p.g_stride[0] + token * p.g_stride[1] + head * p.g_stride[2]) + lane * 16);
+      const uint4 o = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.o) + 2 * (b * p.o_stride[0] + token * p.o_stride[1] + head * p.o_stride[2]) + lane * 16);
+      dot8<BF16>(g, o, dot, norm);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      norm += __shfl_xor_sync(0xffffffffu, norm, o);
+    }
+    norm_g = fmaxf(norm_g, norm);
+    if (lane == 0 && at < rows) {
+      TileRows& t = p.rows[at / kRows];
+      const float lse = valid ? p.lse[(static_cast<size_t>(b) * p.M + token) * p.heads + head] : -INFINITY;
+      t.lse[r] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
+      t.delta[r] = dot;
+      t.doc[r] = p.documents != nullptr && valid ? p.documents[static_cast<size_t>(b) * p.L + pos] : -1;
+      t.slope[r] = p.slopes != nullptr && valid ? p.slopes[head] * 1.4426950408889634f : 0.f;
+      t.pos[r] = static_cast<float>(pos);
+    }
+  }
+  if constexpr (!BF16) {
+    const long long keys = static_cast<long long>(p.batch) * p.L * p.kv_heads;
+    for (long long at = static_cast<long long>(blockIdx.x) * (kRowThreads / 16) + threadIdx.x / 16; at - (threadIdx.x / 16 & 1) < keys; at += step) {
+      const int h = static_cast<int>(at % p.kv_heads), j = static_cast<int>(at / p.kv_heads % p.L), b = static_cast<int>(at / p.kv_heads / p.L);
+      float dot = 0.f, norm = 0.f;
+      if (at < keys && lane < pieces) {
+        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.v) + 2 * (b * p.v_stride[0] + j * p.v_stride[1] + h * p.v_stride[2]) + lane * 16);
+        dot8<BF16>(v, v, dot, norm);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, o);
+      norm_v = fmaxf(norm_v, norm);
+    }
+    // the largest of all: the order of atomics does not show in it
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      norm_g = fmaxf(norm_g, __shfl_xor_sync(0xffffffffu, norm_g, o));
+      norm_v = fmaxf(norm_v, __shfl_xor_sync(0xffffffffu, norm_v, o));
+    }
+    if ((threadIdx.x & 31) == 0) {
+      atomicMax(p.norms, __float_as_uint(norm_g));
+      atomicMax(p.norms + 1, __float_as_uint(norm_v));
+    }
+  }
+}
+
+struct KeySegment {
+  int item, seq, kv_head, block;
+  int lo, hi;               // query tiles
+  int prefix, part, units, at_unit, tile0, valid;
+};
+
+template <int D>
+struct Layout {
+  static constexpr int kAtoms = D / 64, kTile = 128 * D * 2;
+  static constexpr int kOffA = 0, kOffB = kTile;                 // what stays: K and V, or Q and dO
+  static constexpr int kOffRing = 2 * kTile;                     // two stages of what passes: Q and dO, or K and V
+  static constexpr int kOffRows = kOffRing + 4 * kTile;          // [2] TileRows
+  static constexpr int kOffBar = kOffRows + 2 * static_cast<int>(sizeof(TileRows));
+  static constexpr int kOffSeg = kOffBar + 512;
+  static constexpr int kBytes = kOffSeg + 512 + 1024;
+};
+
+struct Bars {
+  uint64_t keep_full, keep_empty;
+  uint64_t full[2], empty[2];
+  uint64_t s_full, s_taken, p_full, dp_full[2], ds_full[2], dp_free[2], acc_done, acc_free;
+  uint64_t seg_full[kSegs], seg_empty[kSegs];
+  uint32_t tmem_base, abort_word;
+  int start_item, start_tile, left, per_cta;
+  int scan[kThreads / 32 + 1];
+};
+static_assert(sizeof(Bars) <= 512, "barrier block too large");
+
+// Query tiles [x, y) that see block j of the keys of batch entry b.
+__device__ __forceinline__ int2 tiles_of_block(const BackwardParams& p, int b, int j) {
+  if (p.documents != nullptr) return p.key_hulls[static_cast<size_t>(b) * p.blocks + j];
+  int first = 0;
+  if (p.causal && !(p.prefix != nullptr && p.prefix[b] > j * kKeys)) first = max(0, j * kKeys - (p.L - p.M));
+  return first < p.M ? make_int2(first / p.tile_tokens, p.tiles) : make_int2(0, 0);
+}
+__device__ __forceinline__ int units_of_item(const BackwardParams& p, int item) {
+  const int j = item % p.blocks, b = item / p.blocks / p.kv_heads;
+  const int2 t = tiles_of_block(p, b, j);
+  return max(1, t.y - t.x);          // (blocks that nobody sees get their zeros)
+}
+
+// The share of this CTA: the tiles of all blocks, in order, in gridDim.x equal shares.
+__device__ __forceinline__ void find_share(const BackwardParams& p, Bars* bar) {
+  constexpr int kWarps = kThreads / 32;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, items = p.batch * p.kv_heads * p.blocks;
+  int sum = 0;
+  for (int i = tid; i < items; i += kThreads) sum += units_of_item(p, i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) bar->scan[warp] = sum;
+  __syncthreads();
+  int total = 0;
+  for (int w = 0; w < kWarps; ++w) total += bar->scan[w];
+  const int grid = gridDim.x, per = max(1, (total + grid - 1) / grid);
+  const int u0 = static_cast<int>(min(static_cast<long long>(per) * blockIdx.x, static_cast<long long>(total))), left = min(per, total - u0);
+  if (tid == 0) bar->left = 0, bar->per_cta = per, bar->start_item = 0, bar->start_tile = 0;
+  int before = 0;
+  for (int base = 0; base < items && before <= u0; base += kThreads) {
+    const int cost = base + tid < items ? units_of_item(p, base + tid) : 0;
+    int incl = cost;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();
+    if (lane == 31) bar->scan[warp] = incl;
+    __syncthreads();
+    int offset = before, all = before;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) offset += bar->scan[w];
+      all += bar->scan[w];
+    }
+    const int at = u0 - (offset + incl - cost);
+    if (left > 0 && at >= 0 && at < cost) bar->start_item = base + tid, bar->start_tile = at, bar->left = left;
+    before = all;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void zero_unused_rows(uint8_t* tile, int atoms, int from) {
+  // rows of a query tile that the loads do not write (a group that does not divide 128): as rows of the sums they have to be zeros
+  for (int a = 0; a < atoms; ++a)
+    for (int i = from * 8 + static_cast<int>(threadIdx.x); i < kRows * 8; i += kThreads)
+      *reinterpret_cast<uint4*>(tile + a * (kRows * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------ gradients of keys and values
+template <int D, bool BF16, bool GENERAL>
+__global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid_constant__ BackwardParams p) {
+  using LO = Layout<D>;
+  constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars* bar = reinterpret_cast<Bars*>(smem + LO::kOffBar);
+  KeySegment* segments = reinterpret_cast<KeySegment*>(smem + LO::kOffSeg);
+  static_assert(sizeof(KeySegment) * kSegs <= 512, "segments");
+  volatile uint32_t* abort_word = &bar->abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar->keep_full, 1);
+    mbar_init(&bar->keep_empty, 2);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 2);
+    }
+    mbar_init(&bar->s_full, 1);
+    mbar_init(&bar->p_full, kComputeWarps);
+    mbar_init(&bar->dp_full[0], 1);
+    mbar_init(&bar->ds_full[0], kComputeWarps);
+    mbar_init(&bar->acc_done, 2);
+    mbar_init(&bar->acc_free, kComputeWarps);
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(&bar->seg_full[i], 1);
+      mbar_init(&bar->seg_empty[i], kComputeWarps + 2);
+    }
+    bar->abort_word = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&bar->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  if (p.group * p.tile_tokens < kRows) {
+    for (int i = 0; i < 4; ++i) zero_unused_rows(smem + LO::kOffRing + i * kTile, kAtoms, p.group * p.tile_tokens);
+    fence_proxy_async_smem();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = bar->tmem_base;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  find_share(p, bar);
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint32_t tile_bytes = static_cast<uint32_t>(p.group * p.tile_tokens) * 128 * kAtoms;
+      int item = bar->start_item, skip = bar->start_tile, left = bar->left, done = 0, n = 0, keeps = 0;
+      bool ok = true;
+      for (int segs = 0; ok; ++segs) {
+        const int slot = segs % kSegs;
+        ok = mbar_wait(&bar->seg_empty[slot], ((segs / kSegs) & 1) ^ 1, abort_word, 0x120);
+        if (!ok) break;
+        KeySegment s;
+        s.valid = left > 0;
+        if (s.valid) {
+          s.item = item;
+          s.block = item % p.blocks;
+          s.kv_head = item / p.blocks % p.kv_heads;
+          s.seq = item / p.blocks / p.kv_heads;
+          const int2 t = tiles_of_block(p, s.seq, s.block);
+          s.units = max(1, t.y - t.x);
+          const int take = min(left, s.units - skip);
+          s.lo = t.x + skip;
+          s.hi = min(t.y, t.x + skip + take);
+          s.part = skip > 0 ? 0 : take < s.units ? 1 : -1;
+          s.at_unit = done;
+          s.prefix = p.prefix != nullptr ? p.prefix[s.seq] : 0;
+          s.tile0 = n;
+          left -= take;
+          done += take;
+          ++item;
+          skip = 0;
+        }
+        segments[slot] = s;
+        mbar_arrive(&bar->seg_full[slot]);
+        if (!s.valid) break;
+        if (s.lo >= s.hi) continue;
+        ok = mbar_wait(&bar->keep_empty, (keeps & 1) ^ 1, abort_word, 0x100);
+        if (!ok) break;
+        ++keeps;
+        mbar_arrive_expect_tx(&bar->keep_full, 2 * kTile);
+        for (int a = 0; a < kAtoms; ++a) {
+          tma_load_4d(smem + LO::kOffA + a * (kKeys * 128), &p.map_k, &bar->keep_full, a * 64, s.block * kKeys, s.kv_head, s.seq);
+          tma_load_4d(smem + LO::kOffB + a * (kKeys * 128), &p.map_v, &bar->keep_full, a * 64, s.block * kKeys, s.kv_head, s.seq);
+        }
+        for (int i = s.lo; i < s.hi; ++i, ++n) {
+          const int st = n & 1;
+          ok = mbar_wait(&bar->empty[st], ((n >> 1) & 1) ^ 1, abort_word, 0x110);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&bar->full[st], 2 * tile_bytes + static_cast<uint32_t>(sizeof(TileRows)));
+          uint8_t* dst = smem + LO::kOffRing + st * 2 * kTile;
+          for (int a = 0; a < kAtoms; ++a) {
+            tma_load_4d(dst + a * (kRows * 128), &p.map_q, &bar->full[st], a * 64, s.kv_head * p.group, i * p.tile_tokens, s.seq);
+            tma_load_4d(dst + kTile + a * (kRows * 128), &p.map_do, &bar->full[st], a * 64, s.kv_head * p.group, i * p.tile_tokens, s.seq);
+          }
+          bulk_load(smem + LO::kOffRows + st * sizeof(TileRows), p.rows + (static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + i,
+                    sizeof(TileRows), &bar->full[st]);
+        }
+      }
+    }
+  } else if (warp >= kMmaWarp) {
+    // ------------------------------------------------------------ MMA: warp 0 S^T = K Q^T and dV += P^T dO, warp 1 dP^T = V dO^T and dK += dS^T Q
+    const int which = warp - kMmaWarp;
+    const uint32_t issuer = elect_one();
+    const uint32_t idesc_s = umma_idesc_f16(BF16, kKeys, kRows, false, false);
+    const uint32_t idesc_acc = umma_idesc_f16(BF16, kKeys, D, false, true);
+    const uint64_t da = umma_desc_sw128(smem_u32(smem + (which == 0 ? LO::kOffA : LO::kOffB)), 16, 1024);
+    // the first product's second operand (Q or dO) K-major, the second product's (dO or Q) with the rows as the reduction
+    const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kTile), 16, 1024);
+    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + (which ^ 1) * kTile), kRows * 128, 1024);
+    const uint32_t d_first = tmem_base + (which == 0 ? kColS : kColDp), d_acc = tmem_base + kColAcc + which * D;
+    uint64_t* first_full = which == 0 ? &bar->s_full : &bar->dp_full[0];
+    uint64_t* back_full = which == 0 ? &bar->p_full : &bar->ds_full[0];
+    auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
+      const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
+      tc_fence_after_sync();
+      return r;
+    };
+    auto issue_first = [&](int n) {
+      const uint64_t db = db0 + (((n & 1) * 2 * kTile) >> 4);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
+        umma_ss_elected(d_first, da + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
+      }
+      umma_commit_elected(first_full, issuer);
+    };
+    uint32_t keeps = 0;
+    int n = 0;
+    bool ok = true;
+    for (int segs = 0; ok; ++segs) {
+      const int slot = segs % kSegs;
+      ok = wait(&bar->seg_full[slot], (segs / kSegs) & 1, 0x350);
+      if (!ok || !segments[slot].valid) break;
+      const int lo = segments[slot].lo, hi = segments[slot].hi;
+      mbar_arrive_warp(&bar->seg_empty[slot], lane);
+      if (lo >= hi) continue;
+      if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300) && wait(&bar->full[n & 1], (n >> 1) & 1, 0x310))) break;
+      issue_first(n);
+      for (int i = lo; i < hi; ++i, ++n) {
+        if (!(ok = wait(back_full, n & 1, 0x340 + which))) break;
+        if (i == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
+        const uint64_t dr = dr0 + (((n & 1) * 2 * kTile) >> 4);
+#pragma unroll
+        for (int k = 0; k < kRows / 16; ++k)
+          umma_ts_elected(d_acc, d_first + (k / 4) * 64 + (k % 4) * 8, dr + ((k * 2048) >> 4), idesc_acc, k > 0 || i > lo ? 1u : 0u, issuer);
+        umma_commit_elected(&bar->empty[n & 1], issuer);
+        if (i + 1 < hi) {
+          if (!(ok = wait(&bar->full[(n + 1) & 1], ((n + 1) >> 1) & 1, 0x311))) break;
+          issue_first(n + 1);
+        }
+      }
+      umma_commit_elected(&bar->keep_empty, issuer);
+      umma_commit_elected(&bar->acc_done, issuer);
+      ++keeps;
+    }
+  } else {
+    // ------------------------------------------------------------ arithmetic: thread a key, half of the tile's rows
+    const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t s_col = lane_base + kColS + half * 64, dp_col = lane_base + kColDp + half * 64;
+    const float c = p.c;
+    float up, down;
+    ds_scale<BF16>(p, &up, &down);
+    const float p_log2 = BF16 ? 0.f : kPScaleLog2, p_down = BF16 ? 1.0f : 1.0f / 16384.0f;
+    const float f = BF16 ? 1.0f : up * p_down;
+    int n = 0;
+    uint32_t accs = 0;
+    bool ok = true;
+    if (threadIdx.x == 0) p.parts[blockIdx.x].last_cta = -1;
+    for (int segs = 0;; ++segs) {
+      const int slot = segs % kSegs;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar->seg_full[slot], (segs / kSegs) & 1, abort_word, 0x840));
+      if (!ok) break;
+      const KeySegment& s = segments[slot];
+      if (!s.valid) break;
+      const int lo = s.lo, hi = s.hi, key = s.block * kKeys + row;
+      int doc = -2;
+      if (GENERAL && p.documents != nullptr && key < p.L) doc = p.documents[static_cast<size_t>(s.seq) * p.L + key];
+      // first column that sees the key: causal, and not in the prefix that all see
+      const bool bounded = p.causal && !(key < s.prefix);
+      for (int i = lo; i < hi; ++i, ++n) {
+        const int st = n & 1;
+        const TileRows& rows = *reinterpret_cast<const TileRows*>(smem + LO::kOffRows + st * sizeof(TileRows));
+        ok = mbar_wait(&bar->full[st], (n >> 1) & 1, abort_word, 0x850);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bar->s_full, n & 1, abort_word, 0x800));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const int from = bounded ? (key - (p.L - p.M) - i * p.tile_tokens) * p.group - half * 64 : 0;      // columns in front of it do not
+        const bool cut = __any_sync(0xffffffffu, from > 0);
+        float w[64];
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t sv[32];
+          tmem_ld_x32_wait(s_col + ch * 32, sv);
+          float g[32];
+          if constexpr (GENERAL) {
+            if (p.cap_out != 0.f) {
+#pragma unroll
+              for (int u = 0; u < 32; ++u) {
+                const float t = tanh_of(__uint_as_float(sv[u]) * p.cap_in);
+                sv[u] = __float_as_uint(p.cap_out * t);
+                g[u] = fmaf(-t, t, 1.0f);
+              }
+            } else {
+#pragma unroll
+              for (int u = 0; u < 32; ++u) g[u] = 1.0f;
+            }
+            if (p.slopes != nullptr) {
+              const float sc = p.cap_out != 0.f ? 1.0f : p.score_log2, at = static_cast<float>(key);
+#pragma unroll
+              for (int u = 0; u < 32; u += 4) {
+                const float4 sl = *reinterpret_cast<const float4*>(&rows.slope[half * 64 + ch * 32 + u]);
+                const float4 ps = *reinterpret_cast<const float4*>(&rows.pos[half * 64 + ch * 32 + u]);
+                sv[u] = __float_as_uint(fmaf(__uint_as_float(sv[u]), sc, -sl.x * fabsf(ps.x - at)));
+                sv[u + 1] = __float_as_uint(fmaf(__uint_as_float(sv[u + 1]), sc, -sl.y * fabsf(ps.y - at)));
+                sv[u + 2] = __float_as_uint(fmaf(__uint_as_float(sv[u + 2]), sc, -sl.z * fabsf(ps.z - at)));
+                sv[u + 3] = __float_as_uint(fmaf(__uint_as_float(sv[u + 3]), sc, -sl.w * fabsf(ps.w - at)));
+              }
+            }
+            if (p.documents != nullptr) {
+#pragma unroll
+              for (int u = 0; u < 32; u += 4) {
+                const int4 d = *reinterpret_cast<const int4*>(&rows.doc[half * 64 + ch * 32 + u]);
+                if (d.x != doc) sv[u] = __float_as_uint(-INFINITY);
+                if (d.y != doc) sv[u + 1] = __float_as_uint(-INFINITY);
+                if (d.z != doc) sv[u + 2] = __float_as_uint(-INFINITY);
+                if (d.w != doc) sv[u + 3] = __float_as_uint(-INFINITY);
+              }
+            }
+          }
+          if (cut) {
+#pragma unroll
+            for (int u = 0; u < 32; ++u)
+              if (ch * 32 + u < from) sv[u] = __float_as_uint(-INFINITY);
+          }
+          const uint64_t c2 = pack_f32x2(c, c);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int v = 0; v < 8; v += 2) {
+              const int u = q * 16 + v * 2;
+              const float4 lse = *reinterpret_cast<const float4*>(&rows.lse[half * 64 + ch * 32 + u]);
+              float p0, p1, p2, p3;
+              unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, pack_f32x2(p_log2 - lse.x, p_log2 - lse.y), false), p0, p1);
+              unpack_f32x2(softmax_weights(sv[u + 2], sv[u + 3], c2, pack_f32x2(p_log2 - lse.z, p_log2 - lse.w), weights_on_fma(u / 2 + 1)), p2, p3);
+              pk[v] = pack2<BF16>(p0, p1);
+              pk[v + 1] = pack2<BF16>(p2, p3);
+              const int x = ch * 32 + u;
+              w[x] = GENERAL ? p0 * g[u] : p0, w[x + 1] = GENERAL ? p1 * g[u + 1] : p1;
+              w[x + 2] = GENERAL ? p2 * g[u + 2] : p2, w[x + 3] = GENERAL ? p3 * g[u + 3] : p3;
+            }
+            // (packed weights go over the first half of this half's own columns)
+            tmem_st_x8(s_col + ch * 16 + q * 8, pk);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive_warp(&bar->p_full, lane);
+
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[0], n & 1, abort_word, 0x810));
+        if (!ok) break;
+        tc_fence_after_sync();
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t dp[32];
+          tmem_ld_x32_wait(dp_col + ch * 32, dp);
+          uint32_t pk[16];
+#pragma unroll
+          for (int u = 0; u < 32; u += 4) {
+            const float4 de = *reinterpret_cast<const float4*>(&rows.delta[half * 64 + ch * 32 + u]);
+            const int x = ch * 32 + u;
+            const float f0 = BF16 ? w[x] : w[x] * f, f1 = BF16 ? w[x + 1] : w[x + 1] * f, f2 = BF16 ? w[x + 2] : w[x + 2] * f,
+                        f3 = BF16 ? w[x + 3] : w[x + 3] * f;
+            pk[u / 2] = pack2<BF16>(f0 * (__uint_as_float(dp[u]) - de.x), f1 * (__uint_as_float(dp[u + 1]) - de.y));
+            pk[u / 2 + 1] = pack2<BF16>(f2 * (__uint_as_float(dp[u + 2]) - de.z), f3 * (__uint_as_float(dp[u + 3]) - de.w));
+          }
+          tmem_st_x16(dp_col + ch * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive_warp(&bar->ds_full[0], lane);
+      }
+      if (!ok) break;
+
+      // the block's gradients, or this part of their sums: dV in the first D columns, dK behind them; half of the columns a thread
+      const bool has = lo < hi;
+      if (has) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->acc_done, accs & 1, abort_word, 0x830));
+        ++accs;
+        if (!ok) break;
+        tc_fence_after_sync();
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float scale = m == 0 ? p_down : p.scale * down;
+        uint8_t* dst = static_cast<uint8_t*>(m == 0 ? p.dv : p.dk) + 2 * ((static_cast<size_t>(s.seq) * p.L + key) * p.kv_heads + s.kv_head) * p.d;
+        float* part = p.part + (((static_cast<size_t>(blockIdx.x) * 2 + max(s.part, 0)) * 2 + m) * kKeys + row) * D;
+#pragma unroll
+        for (int cc = 0; cc < D / 2; cc += 32) {
+          const int col = half * (D / 2) + cc;
+          uint32_t x[32];
+          if (has) {
+            tmem_ld_x32_wait(lane_base + kColAcc + m * D + col, x);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 32; ++u) x[u] = 0u;
+          }
+          if (m == 1 && cc + 32 == D / 2) {
+            tc_fence_before_sync();
+            if (has) mbar_arrive_warp(&bar->acc_free, lane);
+          }
+          if (key >= p.L) continue;
+          if (s.part >= 0) {
+#pragma unroll
+            for (int u = 0; u < 32; u += 4) *reinterpret_cast<uint4*>(part + col + u) = make_uint4(x[u], x[u + 1], x[u + 2], x[u + 3]);
+            continue;
+          }
+#pragma unroll
+          for (int u = 0; u < 32; u += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = pack2<BF16>(__uint_as_float(x[u + 2 * q]) * scale, __uint_as_float(x[u + 2 * q + 1]) * scale);
+            if (col + u < p.d) *reinterpret_cast<uint4*>(dst + 2 * (col + u)) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+      if (s.part == 1 && threadIdx.x == 0) {
+        const long long first_unit = static_cast<long long>(blockIdx.x) * bar->per_cta + s.at_unit;
+        p.parts[blockIdx.x] = {s.item, static_cast<int>((first_unit + s.units - 1) / bar->per_cta)};
+      }
+      mbar_arrive_warp(&bar->seg_empty[slot], lane);
+    }
+  }
+
+  if (bar->abort_word != 0u) {
+    for (int t = 0; t < 64; ++t) __nanosleep(1000);      // loads in flight land before their shared memory is released
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tmem_dealloc(tmem_base, kTmemCols);
+    if (lane == 0 && bar->abort_word != 0 && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(bar->abort_word));
+  }
+}
+
+namespace {
+
+// Sums of the parts of a block that several CTAs had, in the order of its tiles.  One CTA for the block that CTA blockIdx.x began.
+constexpr int kSumThreads = 512;
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kSumThreads, 1) sum_key_parts_kernel(const __grid_constant__ BackwardParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const KeyPartDesc part = p.parts[blockIdx.x];
+  if (part.last_cta < 0) return;
+  const int block = part.item % p.blocks, kv_head = part.item / p.blocks % p.kv_heads, seq = part.item / p.blocks / p.kv_heads;
+  float up, down;
+  ds_scale<BF16>(p, &up, &down);
+  for (int i = threadIdx.x; i < 2 * kKeys * (D / 8); i += kSumThreads) {
+    const int col = i % (D / 8) * 8, row = i / (D / 8) % kKeys, m = i / (D / 8) / kKeys, key = block * kKeys + row;
+    if (key >= p.L || col >= p.d) continue;
+    float x[8] = {};
+    for (int cta = blockIdx.x; cta <= part.last_cta; ++cta) {
+      const float* src = p.part + (((static_cast<size_t>(cta) * 2 + (cta == static_cast<int>(blockIdx.x) ? 1 : 0)) * 2 + m) * kKeys + row) * D + col;
+      const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+      x[0] += a.x, x[1] += a.y, x[2] += a.z, x[3] += a.w, x[4] += b.x, x[5] += b.y, x[6] += b.z, x[7] += b.w;
+    }
+    const float scale = m == 0 ? (BF16 ? 1.0f : 1.0f / 16384.0f) : p.scale * down;
+    uint32_t v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = pack2<BF16>(x[2 * q] * scale, x[2 * q + 1] * scale);
+    uint8_t* dst = static_cast<uint8_t*>(m == 0 ? p.dv : p.dk) + 2 * (((static_cast<size_t>(seq) * p.L + key) * p.kv_heads + kv_head) * p.d + col);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------ gradients of queries
+template <int D, bool BF16, bool GENERAL>
+__global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __grid_constant__ BackwardParams p) {
+  using LO = Layout<D>;
+  constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile;
+  constexpr uint32_t kColDp1 = 384;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars* bar = reinterpret_cast<Bars*>(smem + LO::kOffBar);
+  Segment<1>* segments = reinterpret_cast<Segment<1>*>(smem + LO::kOffSeg);
+  static_assert(sizeof(Segment<1>) * kSegs <= 512, "segments");
+  volatile uint32_t* abort_word = &bar->abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar->keep_full, 1);
+    mbar_init(&bar->keep_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 2);
+      mbar_init(&bar->dp_full[i], 1);
+      mbar_init(&bar->ds_full[i], kComputeWarps);
+      mbar_init(&bar->dp_free[i], 1);
+    }
+    mbar_init(&bar->s_full, 1);
+    mbar_init(&bar->s_taken, kComputeWarps);
+    mbar_init(&bar->acc_done, 1);
+    mbar_init(&bar->acc_free, kComputeWarps);
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(&bar->seg_full[i], 1);
+      mbar_init(&bar->seg_empty[i], kComputeWarps + 2);
+    }
+    bar->abort_word = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&bar->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = bar->tmem_base;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint32_t tile_bytes = static_cast<uint32_t>(p.group * p.tile_tokens) * 128 * kAtoms;
+      DenseWalker<1> walker;
+      Segment<1> s;
+      int n = 0, keeps = 0;
+      bool ok = true;
+      for (int segs = 0; ok; ++segs) {
+        bool more;
+        do {
+          more = walker.next(p, s);
+        } while (more && s.seq < 0);
+        const int slot = segs % kSegs;
+        ok = mbar_wait(&bar->seg_empty[slot], ((segs / kSegs) & 1) ^ 1, abort_word, 0x120);
+        if (!ok) break;
+        s.valid = more;
+        segments[slot] = s;
+        mbar_arrive(&bar->seg_full[slot]);
+        if (!more) break;
+        if (s.lo0 >= s.hi0) continue;
+        ok = mbar_wait(&bar->keep_empty, (keeps & 1) ^ 1, abort_word, 0x100);
+        if (!ok) break;
+        ++keeps;
+        mbar_arrive_expect_tx(&bar->keep_full, 2 * tile_bytes);
+        for (int a = 0; a < kAtoms; ++a) {
+          tma_load_4d(smem + LO::kOffA + a * (kRows * 128), &p.map_q, &bar->keep_full, a * 64, s.kv_head * p.group, s.first_token, s.seq);
+          tma_load_4d(smem + LO::kOffB + a * (kRows * 128), &p.map_do, &bar->keep_full, a * 64, s.kv_head * p.group, s.first_token, s.seq);
+        }
+        for (int j = s.lo0; j < s.hi0; ++j, ++n) {
+          const int st = n & 1;
+          ok = mbar_wait(&bar->empty[st], ((n >> 1) & 1) ^ 1, abort_word, 0x110);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&bar->full[st], 2 * kTile);
+          uint8_t* dst = smem + LO::kOffRing + st * 2 * kTile;
+          for (int a = 0; a < kAtoms; ++a) {
+            tma_load_4d(dst + a * (kKeys * 128), &p.map_k, &bar->full[st], a * 64, j * kKeys, s.kv_head, s.seq);
+            tma_load_4d(dst + kTile + a * (kKeys * 128), &p.map_v, &bar->full[st], a * 64, j * kKeys, s.kv_head, s.seq);
+          }
+        }
+      }
+    }
+  } else if (warp >= kMmaWarp) {
+    // ------------------------------------------------------------ MMA: warp 0 S = Q K^T and dP = dO V^T, warp 1 dQ += dS K
+    const int which = warp - kMmaWarp;
+    const uint32_t issuer = elect_one();
+    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kKeys, false, false);
+    const uint32_t idesc_acc = umma_idesc_f16(BF16, kRows, D, false, true);
+    const uint64_t dq = umma_desc_sw128(smem_u32(smem + LO::kOffA), 16, 1024), ddo = umma_desc_sw128(smem_u32(smem + LO::kOffB), 16, 1024);
+    const uint64_t dk0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing), 16, 1024);
+    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing), kKeys * 128, 1024);
+    auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
+      const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
+      tc_fence_after_sync();
+      return r;
+    };
+    auto scores = [&](uint32_t d, uint64_t a, uint64_t b) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
+        umma_ss_elected(d, a + off, b + off, idesc_s, i > 0 ? 1u : 0u, issuer);
+      }
+    };
+    uint32_t keeps = 0;
+    int n = 0;
+    bool ok = true;
+    for (int segs = 0; ok; ++segs) {
+      const int slot = segs % kSegs;
+      ok = wait(&bar->seg_full[slot], (segs / kSegs) & 1, 0x350);
+      if (!ok || !segments[slot].valid) break;
+      const int lo = segments[slot].lo0, hi = segments[slot].hi0;
+      mbar_arrive_warp(&bar->seg_empty[slot], lane);
+      if (lo >= hi) continue;
+      if (which == 0) {
+        if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300))) break;
+        for (int j = lo; j < hi; ++j, ++n) {
+          const int st = n & 1;
+          const uint32_t two = (n >> 1) & 1;
+          const uint64_t dk = dk0 + ((st * 2 * kTile) >> 4);
+          if (!(ok = wait(&bar->full[st], two, 0x310) && wait(&bar->s_taken, (n & 1) ^ 1, 0x330))) break;
+          scores(tmem_base + kColS, dq, dk);
+          umma_commit_elected(&bar->s_full, issuer);
+          if (!(ok = wait(&bar->dp_free[st], two ^ 1, 0x331))) break;
+          scores(tmem_base + (st ? kColDp1 : kColDp), ddo, dk + (kTile >> 4));
+          umma_commit_elected(&bar->dp_full[st], issuer);
+          umma_commit_elected(&bar->empty[st], issuer);
+        }
+        umma_commit_elected(&bar->keep_empty, issuer);
+      } else {
+        for (int j = lo; j < hi; ++j, ++n) {
+          const int st = n & 1;
+          if (j == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
+          if (!(ok = wait(&bar->ds_full[st], (n >> 1) & 1, 0x340))) break;
+          const uint64_t dr = dr0 + ((st * 2 * kTile) >> 4);
+          const uint32_t a = tmem_base + (st ? kColDp1 : kColDp);
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)
+            umma_ts_elected(tmem_base + kColAcc, a + (k / 4) * 64 + (k % 4) * 8, dr + ((k * 2048) >> 4), idesc_acc, k > 0 || j > lo ? 1u : 0u, issuer);
+          umma_commit_elected(&bar->dp_free[st], issuer);
+          umma_commit_elected(&bar->empty[st], issuer);
+        }
+        umma_commit_elected(&bar->acc_done, issuer);
+      }
+      ++keeps;
+    }
+  } else {
+    // ------------------------------------------------------------ arithmetic: thread a row, half of the block's keys
+    const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    const float c = p.c;
+    float up, down;
+    ds_scale<BF16>(p, &up, &down);
+    const float p_log2 = BF16 ? 0.f : kPScaleLog2, f = BF16 ? 1.0f : up * (1.0f / 16384.0f);
+    const int r_token = row / p.group, r_head = row - r_token * p.group;
+    int n = 0;
+    uint32_t accs = 0;
+    bool ok = true;
+    for (int segs = 0;; ++segs) {
+      const int slot = segs % kSegs;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar->seg_full[slot], (segs / kSegs) & 1, abort_word, 0x840));
+      if (!ok) break;
+      const Segment<1>& s = segments[slot];
+      if (!s.valid) break;
+      const int lo = s.lo0, hi = s.hi0, token = s.first_token + r_token, pos = token + s.keys - s.tokens;
+      const bool valid = r_token < p.tile_tokens && token < s.tokens;
+      const TileRows& rows = p.rows[(static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + s.first_token / p.tile_tokens];
+      const float off = p_log2 - rows.lse[row], delta = rows.delta[row], slope = GENERAL ? rows.slope[row] : 0.f;
+      const int doc = GENERAL ? rows.doc[row] : 0;
+      const int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0;
+      for (int j = lo; j < hi; ++j, ++n) {
+        const int st = n & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full, n & 1, abort_word, 0x800));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const int k0 = j * kKeys + half * 64;
+        const bool cut = __any_sync(0xffffffffu, limit < k0 + 64);
+        float w[64];
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t sv[32];
+          tmem_ld_x32_wait(lane_base + kColS + half * 64 + ch * 32, sv);
+          float g[32];
+          if constexpr (GENERAL) {
+            if (p.cap_out != 0.f) {
+#pragma unroll
+              for (int u = 0; u < 32; ++u) {
+                const float t = tanh_of(__uint_as_float(sv[u]) * p.cap_in);
+                sv[u] = __float_as_uint(p.cap_out * t);
+                g[u] = fmaf(-t, t, 1.0f);
+              }
+            } else {
+#pragma unroll
+              for (int u = 0; u < 32; ++u) g[u] = 1.0f;
+            }
+            if (p.slopes != nullptr) {
+              const float sc = p.cap_out != 0.f ? 1.0f : p.score_log2, far = static_cast<float>(pos - k0 - ch * 32);
+#pragma unroll
+              for (int u = 0; u < 32; ++u)
+                sv[u] = __float_as_uint(fmaf(__uint_as_float(sv[u]), sc, -slope * fabsf(far - static_cast<float>(u))));
+            }
+            if (p.documents != nullptr) {
+              const int only = p.key_blocks[static_cast<size_t>(s.seq) * p.blocks + j].only;
+              if (__any_sync(0xffffffffu, doc >= 0 && doc != only)) {
+                const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
+#pragma unroll
+                for (int u = 0; u < 32; ++u) {
+                  if (ids[min(k0 + ch * 32 + u, p.L - 1)] != doc) sv[u] = __float_as_uint(-INFINITY);
+                  if (u % 8 == 7) asm volatile("" ::: "memory");       // (eight ids at a time: registers)
+                }
+              }
+            }
+          }
+          if (cut) {
+            const int lim = limit - k0 - ch * 32;
+#pragma unroll
+            for (int u = 0; u < 32; ++u)
+              if (u >= lim) sv[u] = __float_as_uint(-INFINITY);
+          }
+          const uint64_t c2 = pack_f32x2(c, c), off2 = pack_f32x2(off, off);
+#pragma unroll
+          for (int u = 0; u < 32; u += 2) {
+            float p0, p1;
+            unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, off2, weights_on_fma(u / 2)), p0, p1);
+            w[ch * 32 + u] = GENERAL ? p0 * g[u] : p0;
+            w[ch * 32 + u + 1] = GENERAL ? p1 * g[u + 1] : p1;
+          }
+        }
+        tc_fence_before_sync();
+        mbar_arrive_warp(&bar->s_taken, lane);
+
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[st], (n >> 1) & 1, abort_word, 0x810));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t dp_col = lane_base + (st ? kColDp1 : kColDp) + half * 64;
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t dp[32], pk[16];
+          tmem_ld_x32_wait(dp_col + ch * 32, dp);
+#pragma unroll
+          for (int u = 0; u < 32; u += 2) {
+            const float w0 = BF16 ? w[ch * 32 + u] : w[ch * 32 + u] * f, w1 = BF16 ? w[ch * 32 + u + 1] : w[ch * 32 + u + 1] * f;
+            pk[u / 2] = pack2<BF16>(w0 * (__uint_as_float(dp[u]) - delta), w1 * (__uint_as_float(dp[u + 1]) - delta));
+          }
+          tmem_st_x16(dp_col + ch * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive_warp(&bar->ds_full[st], lane);
+      }
+      if (!ok) break;
+
+      const bool has = lo < hi;
+      if (has) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->acc_done, accs & 1, abort_word, 0x830));
+        ++accs;
+        if (!ok) break;
+        tc_fence_after_sync();
+      }
+      const float scale = p.scale * down;
+      uint8_t* dst = static_cast<uint8_t*>(p.dq) + 2 * ((static_cast<size_t>(s.seq) * p.M + token) * p.heads + s.kv_head * p.group + r_head) * p.d;
+#pragma unroll
+      for (int cc = 0; cc < D / 2; cc += 32) {
+        const int col = half * (D / 2) + cc;
+        uint32_t x[32];
+        if (has) {
+          tmem_ld_x32_wait(lane_base + kColAcc + col, x);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 32; ++u) x[u] = 0u;
+        }
+        if (cc + 32 == D / 2) {
+          tc_fence_before_sync();
+          if (has) mbar_arrive_warp(&bar->acc_free, lane);
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int u = 0; u < 32; u += 8) {
+          uint32_t v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = pack2<BF16>(__uint_as_float(x[u + 2 * q]) * scale, __uint_as_float(x[u + 2 * q + 1]) * scale);
+          if (col + u < p.d) *reinterpret_cast<uint4*>(dst + 2 * (col + u)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      mbar_arrive_warp(&bar->seg_empty[slot], lane);
+    }
+  }
+
+  if (bar->abort_word != 0u) {
+    for (int t = 0; t < 64; ++t) __nanosleep(1000);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tmem_dealloc(tmem_base, kTmemCols);
+    if (lane == 0 && bar->abort_word != 0 && p.status != nullptr) atomicCAS(p.status, 0, static_cast<int>(bar->abort_word));
+  }
+}
+
+namespace {
+
+cudaLaunchConfig_t config(long long grid, int threads, int smem, cudaStream_t stream, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+template <int D, bool BF16, bool GENERAL>
+cudaError_t launch_products(const BackwardParams& p, int sms, cudaStream_t stream) {
+  auto keys = backward_keys_kernel<D, BF16, GENERAL>;
+  auto queries = backward_queries_kernel<D, BF16, GENERAL>;
+  static std::atomic<unsigned long long> configured{0};
+  int dev = 0;
+  cudaError_t e = current_device_checked(&dev);
+  if (e != cudaSuccess) return e;
+  if (!device_configured(configured, dev)) {
+    e = cudaFuncSetAttribute(keys, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(queries, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes);
+    if (e != cudaSuccess) return e;
+    mark_device_configured(configured, dev);
+  }
+  cudaLaunchAttribute attr[1];
+  e = launch_kernel(config(sms, kThreads, Layout<D>::kBytes, stream, attr), keys, p);
+  if (e == cudaSuccess) e = launch_kernel(config(sms, kSumThreads, 0, stream, attr), sum_key_parts_kernel<D, BF16>, p);
+  if (e == cudaSuccess) e = launch_kernel(config(p.items < sms ? p.items : sms, kThreads, Layout<D>::kBytes, stream, attr), queries, p);
+  return e;
+}
+
+}  // namespace
+
+template <int D, bool BF16>
+cudaError_t launch_backward(const BackwardParams& p, int sms, cudaStream_t stream) {
+  if (!BF16) {
+    const cudaError_t e = cudaMemsetAsync(p.norms, 0, 2 * sizeof(uint32_t), stream);
+    if (e != cudaSuccess) return e;
+  }
+  const long long rows = static_cast<long long>(p.batch) * p.kv_heads * p.tiles * kRows, ctas = (rows + kRowThreads / 16 - 1) / (kRowThreads / 16);
+  cudaLaunchAttribute attr[1];
+  const cudaError_t e = launch_kernel(config(ctas < 8 * sms ? ctas : 8 * sms, kRowThreads, 0, stream, attr), backward_rows_kernel<BF16>, p);
+  if (e != cudaSuccess) return e;
+  const bool general = p.cap_out != 0.f || p.slopes != nullptr || p.documents != nullptr;
+  return general ? launch_products<D, BF16, true>(p, sms, stream) : launch_products<D, BF16, false>(p, sms, stream);
+}
+
+template cudaError_t launch_backward<(DITTO_MASKED_BACKWARD_PART & 1) ? 128 : 64, (DITTO_MASKED_BACKWARD_PART & 2) != 0>(const BackwardParams&, int,
+                                                                                                                       cudaStream_t);
+
+}  // namespace masked
+}  // namespace ditto_b200

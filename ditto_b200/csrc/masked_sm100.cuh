@@ -98,7 +98,8 @@ template <int NT>
 struct DenseWalker {
   int round;
   __device__ __forceinline__ explicit DenseWalker() : round(0) {}
-  __device__ __forceinline__ bool next(const Params& p, Segment<NT>& s) {
+  template <class P>
+  __device__ __forceinline__ bool next(const P& p, Segment<NT>& s) {
     const int grid = gridDim.x, at = round * grid + ((round & 1) ? grid - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
     ++round;
     if (round * grid - grid >= p.items) return false;

@@ -195,6 +195,11 @@ typedef struct {
 /* Scratch bytes that a call needs (0: none); contents irrelevant on entry, undefined on return. */
 size_t ditto_b200_masked_workspace_bytes(const ditto_b200_masked_args* args, int backward);
 int ditto_b200_masked_attention(const ditto_b200_masked_args* args, void* workspace, size_t ws_bytes, int* status_word, void* stream);
+/* Gradients from grad_out [batch, M, heads, head_dim] (strides as above): dq [batch, M, heads, head_dim], dk, dv [batch, L, kv_heads,
+ * head_dim], contiguous, fully written.  args as in the forward call, whose results out and lse are inputs here.  Sums are taken in a fixed
+ * order.  batch x kv_heads x blocks of 128 keys x query tiles is limited to 2^30. */
+int ditto_b200_masked_attention_backward(const ditto_b200_masked_args* args, const void* grad_out, const long long* grad_strides, void* dq,
+                                         void* dk, void* dv, void* workspace, size_t ws_bytes, int* status_word, void* stream);
 
 /* Attention of new tokens over a paged cache that holds their keys and values already.  No counterpart in the reference.
  * Tokens starts[b] .. starts[b + 1] of q (starts NULL: token b) are the last of sequence b's lengths[b] positions; position j of it is slot
