@@ -67,6 +67,14 @@ s3: key_strides value_strides
 ptr: table lengths starts
 ll: table_stride
 int: tokens batch pages page table_cols kv_heads head_dim""")
+PoolsArgs = _block("PoolsArgs", """
+ptr: base
+int: count pages
+ll: page_bytes stride_bytes""")
+TablesArgs = _block("TablesArgs", """
+ptr: table lengths references
+ll: stride
+int: sequences cols page pages""")
 
 EXPORTS = (
     "ditto_b200_bmm_softmax_bmm",
@@ -84,6 +92,12 @@ EXPORTS = (
     "ditto_b200_paged_workspace_bytes",
     "ditto_b200_paged_attention",
     "ditto_b200_cache_append",
+    "ditto_b200_cache_workspace_bytes",
+    "ditto_b200_cache_copy",
+    "ditto_b200_cache_reserve",
+    "ditto_b200_cache_fork",
+    "ditto_b200_cache_free",
+    "ditto_b200_cache_compact",
     "ditto_b200_selftest_umma",
     "ditto_b200_selftest_umma_pair",
     "ditto_b200_selftest_ex2",
@@ -156,6 +170,18 @@ def load():
     lib.ditto_b200_paged_attention.restype = i
     lib.ditto_b200_cache_append.argtypes = [vp, vp, vp]
     lib.ditto_b200_cache_append.restype = i
+    lib.ditto_b200_cache_workspace_bytes.argtypes = [vp, i]
+    lib.ditto_b200_cache_workspace_bytes.restype = sz
+    lib.ditto_b200_cache_copy.argtypes = [vp, vp, vp, i, vp, vp]
+    lib.ditto_b200_cache_copy.restype = i
+    lib.ditto_b200_cache_reserve.argtypes = [vp, vp, vp, sz, vp, vp]
+    lib.ditto_b200_cache_reserve.restype = i
+    lib.ditto_b200_cache_fork.argtypes = [vp, vp, vp, vp, i, vp, sz, vp, vp]
+    lib.ditto_b200_cache_fork.restype = i
+    lib.ditto_b200_cache_free.argtypes = [vp, vp, i, vp, vp]
+    lib.ditto_b200_cache_free.restype = i
+    lib.ditto_b200_cache_compact.argtypes = [vp, vp, vp, ctypes.c_longlong, vp, vp, sz, vp, vp]
+    lib.ditto_b200_cache_compact.restype = i
     lib.ditto_b200_selftest_umma.argtypes = [vp, vp, vp, i, i, i, i, i, vp, vp]
     lib.ditto_b200_selftest_umma.restype = i
     lib.ditto_b200_selftest_umma_pair.argtypes = [vp, vp, vp, i, i, i, i, vp, vp]

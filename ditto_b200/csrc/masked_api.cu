@@ -166,6 +166,43 @@ int check_paged(const ditto_b200_paged_args* a) {
   return check_heads(a->heads, a->kv_heads, a->head_dim, a->dtype);
 }
 
+int check_pools(const ditto_b200_pools* p) {
+  if (!p || !p->base || p->count <= 0 || p->pages <= 0 || p->page_bytes <= 0 || p->stride_bytes < p->page_bytes) return DITTO_ERR_INVALID_ARG;
+  if (p->page_bytes % 16 || p->stride_bytes % 16 || p->page_bytes > (1ll << 32)) return DITTO_ERR_INVALID_ARG;
+  for (int i = 0; i < p->count; ++i)
+    if (!p->base[i] || !aligned16(p->base[i])) return DITTO_ERR_INVALID_ARG;
+  return DITTO_OK;
+}
+
+int check_tables(const ditto_b200_tables* t, bool page_needed, int* status_word, cache::Tables* out) {
+  if (!t || !t->table || !t->references) return DITTO_ERR_INVALID_ARG;
+  if (t->sequences <= 0 || t->cols <= 0 || t->pages <= 0 || t->stride < t->cols || (page_needed && t->page <= 0)) return DITTO_ERR_INVALID_ARG;
+  *out = {t->table, t->lengths, t->references, t->stride, t->sequences, t->cols, t->page, t->pages, status_word};
+  return DITTO_OK;
+}
+
+int copy_pages(const ditto_b200_pools* pools, const int* source, const int* target, const int* n_device, int n, int* status_word, cudaStream_t stream) {
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc) return rc;
+  cache::CopyParams p;
+  p.pools.stride = pools->stride_bytes;
+  p.pools.pieces = static_cast<int>(pools->page_bytes / 16);
+  p.source = source;
+  p.target = target;
+  p.n_device = n_device;
+  p.n = n;
+  p.pages = pools->pages;
+  p.status = status_word;
+  for (int first = 0; first < pools->count; first += cache::kMaxPools) {
+    p.pools.count = pools->count - first < cache::kMaxPools ? pools->count - first : cache::kMaxPools;
+    for (int i = 0; i < p.pools.count; ++i) p.pools.base[i] = static_cast<uint8_t*>(pools->base[first + i]);
+    const cudaError_t e = cache::launch_copy(p, sms, stream);
+    if (e != cudaSuccess) return cuda_fail("cache page copy launch", e);
+  }
+  return DITTO_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -369,6 +406,74 @@ int ditto_b200_cache_append(const ditto_b200_append_args* a, int* status_word, v
   const cudaError_t e = cache::launch_append(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail("cache_append launch", e);
   return DITTO_OK;
+}
+
+int ditto_b200_cache_copy(const ditto_b200_pools* pools, const int* source, const int* target, int n, int* status_word, void* stream) {
+  const int rc = check_pools(pools);
+  if (rc) return rc;
+  if (!source || !target || n <= 0) return DITTO_ERR_INVALID_ARG;
+  return copy_pages(pools, source, target, nullptr, n, status_word, static_cast<cudaStream_t>(stream));
+}
+
+int ditto_b200_cache_free(const ditto_b200_tables* tables, const int* sequences, int n, int* status_word, void* stream) {
+  cache::Tables t;
+  const int rc = check_tables(tables, false, status_word, &t);
+  if (rc) return rc;
+  if (!t.lengths || !sequences || n <= 0) return DITTO_ERR_INVALID_ARG;
+  const cudaError_t e = cache::launch_free(t, sequences, n, static_cast<cudaStream_t>(stream));
+  return e != cudaSuccess ? cuda_fail("cache_free launch", e) : DITTO_OK;
+}
+
+size_t ditto_b200_cache_workspace_bytes(const ditto_b200_tables* t, int n) {
+  if (!t || t->sequences < 0 || t->pages < 0 || n < 0) return 0;
+  // reserve: a word a sequence and one more; fork: three a pair and one; compact: three a page and one
+  const size_t words = 3 * (static_cast<size_t>(t->pages) > static_cast<size_t>(n) ? t->pages : n), seqs = t->sequences;
+  return up256(((words > seqs ? words : seqs) + 1) * sizeof(int));
+}
+
+int ditto_b200_cache_reserve(const ditto_b200_tables* tables, const int* counts, void* workspace, size_t ws_bytes, int* status_word, void* stream) {
+  cache::Tables t;
+  const int rc = check_tables(tables, true, status_word, &t);
+  if (rc) return rc;
+  if (!t.lengths || !counts) return DITTO_ERR_INVALID_ARG;
+  if (!workspace || ws_bytes < (static_cast<size_t>(t.sequences) + 1) * sizeof(int)) return DITTO_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
+  const cudaError_t e = cache::launch_reserve(t, counts, static_cast<int*>(workspace), static_cast<cudaStream_t>(stream));
+  return e != cudaSuccess ? cuda_fail("cache_reserve launch", e) : DITTO_OK;
+}
+
+int ditto_b200_cache_fork(const ditto_b200_pools* pools, const ditto_b200_tables* tables, const int* parents, const int* children, int n,
+                          void* workspace, size_t ws_bytes, int* status_word, void* stream) {
+  cache::Tables t;
+  int rc = check_tables(tables, true, status_word, &t);
+  if (rc == DITTO_OK) rc = check_pools(pools);
+  if (rc) return rc;
+  if (!t.lengths || !parents || !children || n <= 0 || pools->pages != t.pages) return DITTO_ERR_INVALID_ARG;
+  if (!workspace || ws_bytes < (3 * static_cast<size_t>(n) + 1) * sizeof(int)) return DITTO_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
+  int* count = static_cast<int*>(workspace);
+  int *source = count + 1, *target = source + n, *list = target + n;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = cache::launch_fork(t, parents, children, n, source, target, list, count, st);
+  if (e != cudaSuccess) return cuda_fail("cache_fork launch", e);
+  return copy_pages(pools, source, target, count, n, status_word, st);
+}
+
+int ditto_b200_cache_compact(const ditto_b200_pools* pools, const ditto_b200_tables* tables, int* new_table, long long new_stride,
+                             int* new_references, void* workspace, size_t ws_bytes, int* status_word, void* stream) {
+  cache::Tables t;
+  int rc = check_tables(tables, false, status_word, &t);
+  if (rc == DITTO_OK) rc = check_pools(pools);
+  if (rc) return rc;
+  if (!new_table || !new_references || new_stride < t.cols || pools->pages != t.pages) return DITTO_ERR_INVALID_ARG;
+  if (!workspace || ws_bytes < (3 * static_cast<size_t>(t.pages) + 1) * sizeof(int)) return DITTO_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
+  int* count = static_cast<int*>(workspace);
+  int *source = count + 1, *target = source + t.pages, *renamed = target + t.pages;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = cache::launch_compact(t, new_table, new_stride, new_references, renamed, source, target, count, st);
+  if (e != cudaSuccess) return cuda_fail("cache_compact launch", e);
+  return copy_pages(pools, source, target, count, t.pages, status_word, st);
 }
 
 }  // extern "C"

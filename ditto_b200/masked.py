@@ -230,19 +230,23 @@ def _check_cache(key_pages, value_pages, block_table, lengths, query_starts, dty
 
 
 def _check_table(block_table, lengths, device):
-    if not isinstance(block_table, torch.Tensor) or not block_table.is_cuda:
-        raise TypeError("block_table must be a CUDA tensor (ditto_b200 has no CPU path)")
-    if block_table.dtype != torch.int32:
-        raise TypeError(f"block_table has dtype {block_table.dtype}, expected torch.int32")
-    if block_table.dim() != 2 or (block_table.numel() and block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError("block_table must be 2-D with contiguous rows")
-    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
-        raise ValueError("block_table: rows overlap")
-    if device is not None and block_table.device != device:
-        raise ValueError(f"block_table is on {block_table.device}, expected {device}")
+    _check_rows(block_table, device)
     _check(lengths, "lengths", torch.int32, block_table.device, 1)
     if block_table.shape[0] != lengths.shape[0]:
         raise ValueError(f"block_table has {block_table.shape[0]} rows, lengths {lengths.shape[0]} values")
+
+
+def _check_rows(block_table, device, name="block_table"):
+    if not isinstance(block_table, torch.Tensor) or not block_table.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor (ditto_b200 has no CPU path)")
+    if block_table.dtype != torch.int32:
+        raise TypeError(f"{name} has dtype {block_table.dtype}, expected torch.int32")
+    if block_table.dim() != 2 or (block_table.numel() and block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"{name} must be 2-D with contiguous rows")
+    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError(f"{name}: rows overlap")
+    if device is not None and block_table.device != device:
+        raise ValueError(f"{name} is on {block_table.device}, expected {device}")
 
 
 def paged_attention(query, key_pages, value_pages, block_table, lengths, query_starts=None, out=None, scale=1.0, prefix=None, slopes=None,

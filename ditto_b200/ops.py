@@ -393,5 +393,6 @@ def ffn(x, w1, b1, w2, b2, out=None, act1="relu", act2="relu", weight_layout="OI
     return out
 
 
-# attention with masks and modified scores, and over a paged cache (they use what this module defines)
+# attention with masks and modified scores, over a paged cache, and the cache's pages (they use what this module defines)
+from .cache import cache_compact, cache_copy, cache_fork, cache_free, cache_reserve  # noqa: E402,F401
 from .masked import cache_append, masked_attention, masked_attention_backward, paged_attention  # noqa: E402,F401

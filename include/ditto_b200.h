@@ -238,6 +238,39 @@ typedef struct {
 } ditto_b200_append_args;
 int ditto_b200_cache_append(const ditto_b200_append_args* args, int* status_word, void* stream);
 
+/* Pages of a cache.  No counterpart in the reference.  Pools (the keys and the values of every layer) share one numbering of pages; a table
+ * row lists a sequence's pages, -1 where it has none; references[page] counts the table entries that name a page, 0 for a free one.  Everything
+ * is read and written on the device, in stream order, so that calls can be captured; free pages are taken lowest first, so that
+ * the same tables give the same tables.  Ids out of range are passed over and store DITTO_STATUS_BAD_PAGE. */
+typedef struct {
+  void* const* base;       /* host array of count device addresses, 16-byte aligned */
+  int count, pages;
+  long long page_bytes;    /* contiguous, a multiple of 16 */
+  long long stride_bytes;  /* from page to page, the same in all pools */
+} ditto_b200_pools;
+typedef struct {
+  int *table, *lengths, *references;   /* [sequences, cols], [sequences] (compact: NULL), [pages] */
+  long long stride;                    /* entries between rows of the table */
+  int sequences, cols, page, pages;    /* page: positions a page (free and compact do not need it) */
+} ditto_b200_tables;
+/* Scratch bytes for reserve, fork (n pairs) and compact. */
+size_t ditto_b200_cache_workspace_bytes(const ditto_b200_tables* tables, int n);
+/* Copies page source[i] to target[i] in every pool; a negative id: no copy.  No target may be another target or a source. */
+int ditto_b200_cache_copy(const ditto_b200_pools* pools, const int* source, const int* target, int n, int* status_word, void* stream);
+/* lengths[s] += counts[s], with the new pages that takes; all or nothing: where there are not enough free pages, or columns, nothing changes
+ * and DITTO_STATUS_NO_PAGES is stored. */
+int ditto_b200_cache_reserve(const ditto_b200_tables* tables, const int* counts, void* workspace, size_t ws_bytes, int* status_word, void* stream);
+/* Sequence children[i] becomes a copy of parents[i]: full pages are shared, a last page that is not full is copied to a free one.  Children
+ * are sequences without pages, all different, none a parent.  All or nothing as above. */
+int ditto_b200_cache_fork(const ditto_b200_pools* pools, const ditto_b200_tables* tables, const int* parents, const int* children, int n,
+                          void* workspace, size_t ws_bytes, int* status_word, void* stream);
+/* Gives the sequences' pages back: their rows become -1, their lengths 0.  The same sequence twice counts once. */
+int ditto_b200_cache_free(const ditto_b200_tables* tables, const int* sequences, int n, int* status_word, void* stream);
+/* Moves the live pages to the front of the pools; the table and references that go with it are written to new_table and new_references, which
+ * may be the old ones.  With n live pages the k-th of those behind the first n goes to the k-th free place among them. */
+int ditto_b200_cache_compact(const ditto_b200_pools* pools, const ditto_b200_tables* tables, int* new_table, long long new_stride,
+                             int* new_references, void* workspace, size_t ws_bytes, int* status_word, void* stream);
+
 /* Single-CTA check of one tcgen05 MMA chain: c[128, N] (fp32) = a[128, K] * b.
  *   b_mn 0: b is [N, K]; 1: b is [K, N].  a_tmem 1: the A operand is read from tensor memory.
  * N, K multiples of 64, at most 256.  Exists so the descriptor encodings the fused kernels depend
