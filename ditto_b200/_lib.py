@@ -109,6 +109,9 @@ EXPORTS = (
     "ditto_b200_version",
 )
 
+# masked attention, the paged cache and its pages
+MASKED_EXPORTS = tuple(name for name in EXPORTS if "masked" in name or "paged" in name or "_cache_" in name)
+
 
 class DittoError(RuntimeError):
     """A non-zero status from the C ABI."""

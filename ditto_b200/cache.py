@@ -67,6 +67,7 @@ def _call(name, device, *args):
     with _ops._on_device(device):
         rc = getattr(lib, name)(*args, _ops._status_ptr(device), torch.cuda.current_stream().cuda_stream)
     _lib.check(rc, name)
+    _ops._enable_fast(device)
     _ops.launch_count += 1
 
 
@@ -109,6 +110,9 @@ def cache_fork(pools, block_table, lengths, references, parents, children, page_
     """Sequence children[i] becomes a copy of sequence parents[i] (int32, on the device): it shares the full pages and gets a copy of a last page
     that is not full, in the lowest free page.  Children are sequences without pages, all different, none a parent; a parent may have any
     number of them.  All or nothing as in cache_reserve."""
+    if _ops._fast is not None and _ops._fast.cache_fork(pools, block_table, lengths, references, parents, children, page_size):
+        _ops.launch_count += 1
+        return
     t = _tables(block_table, lengths, references, page_size)
     device = block_table.device
     n = _ids(parents, "parents", device)
@@ -126,6 +130,9 @@ def cache_fork(pools, block_table, lengths, references, parents, children, page_
 
 def cache_free(block_table, lengths, references, sequences):
     """Gives back the pages of the sequences (int32, on the device): rows become -1, lengths 0.  A sequence that is named twice is freed once."""
+    if _ops._fast is not None and _ops._fast.cache_free(block_table, lengths, references, sequences):
+        _ops.launch_count += 1
+        return
     t = _tables(block_table, lengths, references, None)
     n = _ids(sequences, "sequences", block_table.device)
     if n and t.sequences:
@@ -137,6 +144,11 @@ def cache_compact(pools, block_table, references, out_table=None, out_references
     """Moves the live pages to the front of the pools and returns the table and the references that go with it (new tensors, or out_table and
     out_references, which may be the old ones).  With n live pages the k-th of those behind the first n goes to the k-th free place among
     them; the pages that are left keep their contents."""
+    if _ops._fast is not None and out_table is None and out_references is None:
+        r = _ops._fast.cache_compact(pools, block_table, references)
+        if r is not None:
+            _ops.launch_count += 1
+            return r
     _masked._check_rows(block_table, None)
     device = block_table.device
     _masked._check(references, "references", torch.int32, device, 1)

@@ -16,13 +16,19 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include "../../include/ditto_b200.h"
 
 #include <algorithm>
 #include <climits>
 #include <cstring>
 #include <initializer_list>
+#include <string_view>
+#include <type_traits>
+#include <vector>
 
 namespace {
 
@@ -89,6 +95,14 @@ void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast
 
 bool shape_is(const at::Tensor& t, int64_t a, int64_t b, int64_t c) {
   return t.dim() == 3 && t.size(0) == a && t.size(1) == b && t.size(2) == c;
+}
+
+// A pair of two new references.
+PyObject* pair_of(PyObject* first, PyObject* second) {
+  PyObject* t = PyTuple_New(2);
+  PyTuple_SET_ITEM(t, 0, first);
+  PyTuple_SET_ITEM(t, 1, second);
+  return t;
 }
 
 // Lets other Python threads run: around allocations and launches, which can block (a full launch queue, cudaMalloc, a queue that
@@ -364,6 +378,420 @@ PyObject* py_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------------------ masked attention and the paged cache
+// Entry points by their declared types, bound by name (bind_masked).
+struct Masked {
+  decltype(&ditto_b200_masked_workspace_bytes) bytes = nullptr;
+  decltype(&ditto_b200_masked_attention) forward = nullptr;
+  decltype(&ditto_b200_masked_attention_backward) backward = nullptr;
+  decltype(&ditto_b200_paged_workspace_bytes) paged_bytes = nullptr;
+  decltype(&ditto_b200_paged_attention) paged = nullptr;
+  decltype(&ditto_b200_cache_append) append = nullptr;
+  decltype(&ditto_b200_cache_workspace_bytes) cache_bytes = nullptr;
+  decltype(&ditto_b200_cache_fork) fork = nullptr;
+  decltype(&ditto_b200_cache_free) free = nullptr;
+  decltype(&ditto_b200_cache_compact) compact = nullptr;
+} g_masked;
+
+// A 16-bit CUDA tensor of `dims` dimensions, not empty, its last one contiguous, the data and the other strides multiples of 16 bytes; the
+// strides go to `strides` (dimensions of one entry: any valid one).
+const at::Tensor* take_strided(PyObject* o, Common& c, int dims, long long* strides) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() != dims || t.numel() == 0) return nullptr;
+  const int dev = t.device().index();
+  const at::ScalarType st = t.scalar_type();
+  if (c.device < 0) {
+    if (st == at::kHalf) c.code = 0;
+    else if (st == at::kBFloat16) c.code = 1;
+    else return nullptr;
+    if (dev < 0 || dev >= kDevices || g_status[dev] == nullptr || dev != c10::cuda::current_device()) return nullptr;
+    c.device = dev;
+    c.type = st;
+  } else if (dev != c.device || st != c.type) {
+    return nullptr;
+  }
+  if (t.stride(dims - 1) != 1 && t.size(dims - 1) != 1) return nullptr;
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return nullptr;
+  for (int i = 0; i + 1 < dims; ++i) {
+    if (t.size(i) > INT_MAX) return nullptr;
+    if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8)) return nullptr;
+    if (strides != nullptr) strides[i] = t.size(i) > 1 ? t.stride(i) : 8;
+  }
+  return &t;
+}
+
+// A contiguous CUDA tensor of another type on the call's device, of this many entries in its one dimension (below 0: any number).
+const at::Tensor* take_vector(PyObject* o, int device, at::ScalarType type, int64_t n) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.device().index() != device || t.scalar_type() != type || t.dim() != 1 || !t.is_contiguous()) return nullptr;
+  return n < 0 || t.size(0) == n ? &t : nullptr;
+}
+// ... or None: *out is its address or null.
+template <class T>
+bool optional_vector(PyObject* o, int device, at::ScalarType type, int64_t n, const T** out) {
+  *out = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = take_vector(o, device, type, n);
+  if (t == nullptr || t->requires_grad()) return false;
+  *out = static_cast<const T*>(t->data_ptr());
+  return true;
+}
+// A table of page ids with contiguous rows.
+const at::Tensor* take_table(PyObject* o, int device) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.device().index() != device || t.scalar_type() != at::kInt || t.dim() != 2 || t.numel() == 0 || t.stride(1) != 1) return nullptr;
+  if (t.size(0) > 1 && t.stride(0) < t.size(1)) return nullptr;
+  return t.size(0) <= INT_MAX && t.size(1) <= INT_MAX ? &t : nullptr;
+}
+long long row_stride(const at::Tensor& t) { return std::max<int64_t>(t.stride(0), t.size(1)); }
+
+bool number(PyObject* o, float* out) {
+  const double v = PyFloat_AsDouble(o);
+  *out = static_cast<float>(v);
+  return !(v == -1.0 && PyErr_Occurred());
+}
+bool optional_cap(PyObject* o, float* out) {
+  *out = 0.f;
+  return o == Py_None || (number(o, out) && *out > 0.f);
+}
+
+at::Tensor workspace(size_t bytes, int device) {
+  return bytes == 0 ? at::Tensor() : make({static_cast<int64_t>(bytes)}, at::kByte, device);
+}
+
+// The operands and rules from the arguments  q, k, v, out (may be None), scale, causal, prefix, documents, slopes, cap.
+bool masked_args(PyObject* const* a, Common& c, ditto_b200_masked_args& r, const at::Tensor** query, const at::Tensor** key, const at::Tensor** out) {
+  const at::Tensor* q = take_strided(a[0], c, 4, r.q_strides);
+  const at::Tensor* k = q ? take_strided(a[1], c, 4, r.k_strides) : nullptr;
+  const at::Tensor* v = k ? take_strided(a[2], c, 4, r.v_strides) : nullptr;
+  if (v == nullptr || k->sizes() != v->sizes() || k->size(0) != q->size(0) || k->size(3) != q->size(3)) return false;
+  *out = nullptr;
+  if (a[3] != Py_None && ((*out = take_strided(a[3], c, 4, r.out_strides)) == nullptr || (*out)->sizes() != q->sizes())) return false;
+  r.batch = q->size(0), r.M = q->size(1), r.heads = q->size(2), r.head_dim = q->size(3), r.L = k->size(1), r.kv_heads = k->size(2);
+  r.dtype = c.code;
+  if (r.kv_heads == 0 || r.heads % r.kv_heads) return false;
+  if (!number(a[4], &r.scale) || !optional_cap(a[9], &r.cap)) return false;
+  if (a[5] != Py_True && a[5] != Py_False) return false;
+  r.causal = a[5] == Py_True;
+  if (!optional_vector(a[6], c.device, at::kInt, r.batch, &r.prefix) || !optional_vector(a[8], c.device, at::kFloat, r.heads, &r.slopes)) return false;
+  r.documents = nullptr;
+  if (a[7] != Py_None) {
+    const at::Tensor* d = take_table(a[7], c.device);
+    if (d == nullptr || !d->is_contiguous() || d->size(0) != r.batch || d->size(1) != r.L) return false;
+    r.documents = static_cast<const int*>(d->data_ptr());
+  }
+  r.q = q->data_ptr(), r.k = k->data_ptr(), r.v = v->data_ptr();
+  r.out = *out ? (*out)->data_ptr() : nullptr;
+  *query = q, *key = k;
+  return true;
+}
+void compact_strides(const at::Tensor& t, long long* strides) {
+  for (int i = 0; i < 3; ++i) strides[i] = t.size(i) > 1 ? t.stride(i) : 8;
+}
+
+// masked(query, key, value, out, scale, causal, prefix, documents, slopes, cap, return_lse)
+PyObject* py_masked(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 11 || g_masked.forward == nullptr) return nullptr;
+    Common c;
+    ditto_b200_masked_args r = {};
+    const at::Tensor *q, *k, *given;
+    if (!masked_args(a, c, r, &q, &k, &given)) return nullptr;
+    if (c10::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || THPVariable_Unpack(a[2]).requires_grad())) return nullptr;
+    const bool want_lse = a[10] == Py_True;
+    at::Tensor out, lse;
+    const std::vector<int64_t> shape = q->sizes().vec();
+    int rc;
+    {
+      WithoutLock unlocked;
+      if (given == nullptr) {
+        out = make(shape, c.type, c.device);
+        r.out = out.data_ptr();
+        compact_strides(out, r.out_strides);
+      }
+      if (want_lse) {
+        lse = make(at::IntArrayRef(shape.data(), 3), at::kFloat, c.device);
+        r.lse = static_cast<float*>(lse.data_ptr());
+      }
+      const size_t bytes = r.documents != nullptr ? g_masked.bytes(&r, 0) : 0;
+      at::Tensor ws = workspace(bytes, c.device);
+      rc = g_masked.forward(&r, bytes ? ws.data_ptr() : nullptr, bytes, g_status[c.device], stream_of(c.device));
+    }
+    if (rc) return nullptr;
+    PyObject* first = a[3];
+    if (given == nullptr) first = THPVariable_Wrap(out);
+    else Py_INCREF(first);
+    if (!want_lse) return first;
+    return pair_of(first, THPVariable_Wrap(lse));
+  });
+}
+
+// masked_backward(grad_out, query, key, value, out, lse, scale, causal, prefix, documents, slopes, cap) -> (dq, dk, dv)
+PyObject* py_masked_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 12 || g_masked.backward == nullptr || a[4] == Py_None) return nullptr;
+    Common c;
+    ditto_b200_masked_args r = {};
+    const at::Tensor *q, *k, *out;
+    PyObject* const args[10] = {a[1], a[2], a[3], a[4], a[6], a[7], a[8], a[9], a[10], a[11]};
+    if (!masked_args(args, c, r, &q, &k, &out)) return nullptr;
+    long long strides[3];
+    const at::Tensor* g = take_strided(a[0], c, 4, strides);
+    if (g == nullptr || g->sizes() != q->sizes() || !THPVariable_Check(a[5])) return nullptr;
+    const at::Tensor& lse = THPVariable_Unpack(a[5]);
+    if (!lse.is_cuda() || lse.device().index() != c.device || lse.scalar_type() != at::kFloat || !lse.is_contiguous() ||
+        !shape_is(lse, r.batch, r.M, r.heads))
+      return nullptr;
+    r.lse = static_cast<float*>(lse.data_ptr());
+    const void* gp = g->data_ptr();
+    const std::vector<int64_t> rows = q->sizes().vec(), keys = k->sizes().vec();
+    at::Tensor dq, dk, dv;
+    int rc;
+    {
+      WithoutLock unlocked;
+      dq = make(rows, c.type, c.device);
+      dk = make(keys, c.type, c.device);
+      dv = make(keys, c.type, c.device);
+      const size_t bytes = g_masked.bytes(&r, 1);
+      at::Tensor ws = workspace(bytes, c.device);
+      rc = g_masked.backward(&r, gp, strides, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
+                             g_status[c.device], stream_of(c.device));
+    }
+    if (rc) return nullptr;
+    PyObject* t = PyTuple_New(3);
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(dq));
+    PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(dk));
+    PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(dv));
+    return t;
+  });
+}
+
+// The cache of a call: key_pages, value_pages, block_table, lengths, query_starts (or None).
+struct Cache {
+  const at::Tensor *keys, *values, *table;
+  const int *lengths, *starts;
+  int batch;
+};
+bool cache_of(PyObject* const* a, Common& c, int64_t tokens, long long* key_strides, long long* value_strides, Cache& r) {
+  r.keys = take_strided(a[0], c, 4, key_strides);
+  r.values = r.keys ? take_strided(a[1], c, 4, value_strides) : nullptr;
+  if (r.values == nullptr || r.keys->sizes() != r.values->sizes() || (r.table = take_table(a[2], c.device)) == nullptr) return false;
+  r.batch = static_cast<int>(r.table->size(0));
+  const at::Tensor* lengths = take_vector(a[3], c.device, at::kInt, r.batch);
+  if (lengths == nullptr || !optional_vector(a[4], c.device, at::kInt, r.batch + 1, &r.starts)) return false;
+  r.lengths = static_cast<const int*>(lengths->data_ptr());
+  return r.starts != nullptr || tokens == r.batch;
+}
+
+// paged(query, key_pages, value_pages, block_table, lengths, query_starts, out, scale, prefix, slopes, cap)
+PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 11 || g_masked.paged == nullptr) return nullptr;
+    Common c;
+    ditto_b200_paged_args r = {};
+    Cache cache;
+    const at::Tensor* q = take_strided(a[0], c, 3, r.q_strides);
+    if (q == nullptr || !cache_of(a + 1, c, q->size(0), r.key_strides, r.value_strides, cache) || cache.keys->size(3) != q->size(2)) return nullptr;
+    const at::Tensor* given = nullptr;
+    if (a[6] != Py_None && ((given = take_strided(a[6], c, 3, r.out_strides)) == nullptr || given->sizes() != q->sizes())) return nullptr;
+    r.tokens = q->size(0), r.heads = q->size(1), r.head_dim = q->size(2), r.batch = cache.batch;
+    r.pages = cache.keys->size(0), r.page = cache.keys->size(1), r.kv_heads = cache.keys->size(2);
+    r.table_cols = cache.table->size(1), r.table_stride = row_stride(*cache.table), r.dtype = c.code;
+    if (!number(a[7], &r.scale) || !optional_cap(a[10], &r.cap) || !optional_vector(a[8], c.device, at::kInt, r.batch, &r.prefix) ||
+        !optional_vector(a[9], c.device, at::kFloat, r.heads, &r.slopes))
+      return nullptr;
+    r.q = q->data_ptr(), r.key_pages = cache.keys->data_ptr(), r.value_pages = cache.values->data_ptr();
+    r.table = static_cast<const int*>(cache.table->data_ptr()), r.lengths = cache.lengths, r.starts = cache.starts;
+    r.out = given ? given->data_ptr() : nullptr;
+    const int64_t shape[3] = {r.tokens, r.heads, r.head_dim};
+    at::Tensor out;
+    int rc;
+    {
+      WithoutLock unlocked;
+      if (given == nullptr) {
+        out = make(shape, c.type, c.device);
+        if (r.starts != nullptr) out.zero_();          // (tokens of no sequence)
+        r.out = out.data_ptr();
+        for (int i = 0; i < 2; ++i) r.out_strides[i] = shape[i] > 1 ? out.stride(i) : 8;
+      }
+      const size_t bytes = g_masked.paged_bytes(&r);
+      at::Tensor ws = workspace(bytes, c.device);
+      rc = g_masked.paged(&r, bytes ? ws.data_ptr() : nullptr, bytes, g_status[c.device], stream_of(c.device));
+    }
+    if (rc) return nullptr;
+    if (given == nullptr) return THPVariable_Wrap(out);
+    Py_INCREF(a[6]);
+    return a[6];
+  });
+}
+
+// append(keys, values, key_pages, value_pages, block_table, lengths, query_starts) -> True
+PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 7 || g_masked.append == nullptr) return nullptr;
+    Common c;
+    ditto_b200_append_args r = {};
+    Cache cache;
+    const at::Tensor *k = take_strided(a[0], c, 3, r.k_strides), *v = k ? take_strided(a[1], c, 3, r.v_strides) : nullptr;
+    if (v == nullptr || k->sizes() != v->sizes() || !cache_of(a + 2, c, k->size(0), r.key_strides, r.value_strides, cache)) return nullptr;
+    if (cache.keys->size(2) != k->size(1) || cache.keys->size(3) != k->size(2)) return nullptr;
+    r.keys = k->data_ptr(), r.values = v->data_ptr(), r.key_pages = cache.keys->data_ptr(), r.value_pages = cache.values->data_ptr();
+    r.table = static_cast<const int*>(cache.table->data_ptr()), r.lengths = cache.lengths, r.starts = cache.starts;
+    r.table_stride = row_stride(*cache.table), r.table_cols = cache.table->size(1);
+    r.tokens = k->size(0), r.batch = cache.batch, r.kv_heads = k->size(1), r.head_dim = k->size(2);
+    r.pages = cache.keys->size(0), r.page = cache.keys->size(1);
+    int rc;
+    {
+      WithoutLock unlocked;
+      rc = g_masked.append(&r, g_status[c.device], stream_of(c.device));
+    }
+    if (rc) return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// The tables of a cache; lengths may be null where the call does not need them.
+bool tables_of(PyObject* table, PyObject* lengths, PyObject* references, int* device, ditto_b200_tables& r) {
+  if (!THPVariable_Check(table)) return false;
+  *device = THPVariable_Unpack(table).device().index();
+  if (*device < 0 || *device >= kDevices || g_status[*device] == nullptr || *device != c10::cuda::current_device()) return false;
+  const at::Tensor* t = take_table(table, *device);
+  if (t == nullptr) return false;
+  const at::Tensor* l = lengths ? take_vector(lengths, *device, at::kInt, t->size(0)) : nullptr;
+  const at::Tensor* f = take_vector(references, *device, at::kInt, -1);
+  if ((lengths && l == nullptr) || f == nullptr || f->size(0) == 0 || f->size(0) > INT_MAX) return false;
+  r.table = static_cast<int*>(t->data_ptr()), r.lengths = l ? static_cast<int*>(l->data_ptr()) : nullptr;
+  r.references = static_cast<int*>(f->data_ptr());
+  r.stride = row_stride(*t), r.sequences = t->size(0), r.cols = t->size(1), r.page = 0, r.pages = f->size(0);
+  return true;
+}
+// Pools [pages, ...] of one shape, type and stride, in a list or tuple.
+bool pools_of(PyObject* o, int device, int64_t pages, std::vector<void*>& base, ditto_b200_pools& r) {
+  if (!PyList_Check(o) && !PyTuple_Check(o)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  if (n == 0) return false;
+  const at::Tensor* first = nullptr;
+  base.resize(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* x = PySequence_Fast_GET_ITEM(o, i);
+    if (!THPVariable_Check(x)) return false;
+    const at::Tensor& t = THPVariable_Unpack(x);
+    if (!t.is_cuda() || t.device().index() != device || t.dim() < 2) return false;
+    if (first == nullptr) {
+      first = &t;
+      if (t.size(0) != pages || t.numel() == 0) return false;
+      int64_t inner = 1;                               // a page is contiguous
+      for (int64_t d = t.dim() - 1; d > 0; --d) {
+        if (t.size(d) != 1 && t.stride(d) != inner) return false;
+        inner *= t.size(d);
+      }
+      r.page_bytes = inner * t.element_size();
+      r.stride_bytes = t.size(0) > 1 ? t.stride(0) * static_cast<int64_t>(t.element_size()) : r.page_bytes;
+    } else if (t.sizes() != first->sizes() || t.strides() != first->strides() || t.scalar_type() != first->scalar_type()) {
+      return false;
+    }
+    base[i] = t.data_ptr();
+  }
+  r.base = base.data(), r.count = static_cast<int>(n), r.pages = static_cast<int>(pages);
+  return true;
+}
+
+// cache_free(block_table, lengths, references, sequences) -> True
+PyObject* py_cache_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int device;
+    ditto_b200_tables t;
+    if (n != 4 || g_masked.free == nullptr || !tables_of(a[0], a[1], a[2], &device, t)) return nullptr;
+    const at::Tensor* s = take_vector(a[3], device, at::kInt, -1);
+    if (s == nullptr || s->size(0) == 0 || s->size(0) > INT_MAX) return nullptr;
+    const int* sp = static_cast<const int*>(s->data_ptr());
+    const int count = static_cast<int>(s->size(0));
+    int rc;
+    {
+      WithoutLock unlocked;
+      rc = g_masked.free(&t, sp, count, g_status[device], stream_of(device));
+    }
+    if (rc) return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// cache_fork(pools, block_table, lengths, references, parents, children, page_size) -> True
+PyObject* py_cache_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int device;
+    ditto_b200_tables t;
+    ditto_b200_pools pools;
+    std::vector<void*> base;
+    if (n != 7 || g_masked.fork == nullptr || !tables_of(a[1], a[2], a[3], &device, t) || !pools_of(a[0], device, t.pages, base, pools)) return nullptr;
+    const at::Tensor *from = take_vector(a[4], device, at::kInt, -1), *to = from ? take_vector(a[5], device, at::kInt, from->size(0)) : nullptr;
+    if (to == nullptr || to->size(0) == 0 || to->size(0) > t.sequences) return nullptr;
+    const long page = PyLong_AsLong(a[6]);
+    if (page <= 0 || page > INT_MAX) return nullptr;
+    t.page = static_cast<int>(page);
+    const int *fp = static_cast<const int*>(from->data_ptr()), *tp = static_cast<const int*>(to->data_ptr());
+    const int count = static_cast<int>(to->size(0));
+    int rc;
+    {
+      WithoutLock unlocked;
+      const size_t bytes = g_masked.cache_bytes(&t, count);
+      at::Tensor ws = workspace(bytes, device);
+      rc = g_masked.fork(&pools, &t, fp, tp, count, ws.data_ptr(), bytes, g_status[device], stream_of(device));
+    }
+    if (rc) return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// cache_compact(pools, block_table, references) -> (table, references)
+PyObject* py_cache_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    int device;
+    ditto_b200_tables t;
+    ditto_b200_pools pools;
+    std::vector<void*> base;
+    if (n != 3 || g_masked.compact == nullptr || !tables_of(a[1], nullptr, a[2], &device, t) || !pools_of(a[0], device, t.pages, base, pools)) return nullptr;
+    at::Tensor table, references;
+    int rc;
+    {
+      WithoutLock unlocked;
+      table = make({t.sequences, t.cols}, at::kInt, device);
+      references = make({t.pages}, at::kInt, device);
+      const size_t bytes = g_masked.cache_bytes(&t, 0);
+      at::Tensor ws = workspace(bytes, device);
+      rc = g_masked.compact(&pools, &t, static_cast<int*>(table.data_ptr()), t.cols, static_cast<int*>(references.data_ptr()), ws.data_ptr(), bytes,
+                            g_status[device], stream_of(device));
+    }
+    if (rc) return nullptr;
+    return pair_of(THPVariable_Wrap(table), THPVariable_Wrap(references));
+  });
+}
+
+// bind_masked(name, address): a C entry point of the operators above
+PyObject* py_bind_masked(PyObject*, PyObject* args) {
+  const char* name;
+  unsigned long long p;
+  if (!PyArg_ParseTuple(args, "sK", &name, &p)) return nullptr;
+  const std::string_view s(name);
+  auto set = [&](const char* known, auto& fn) {
+    if (s == known) fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(p);
+  };
+  set("ditto_b200_masked_workspace_bytes", g_masked.bytes);
+  set("ditto_b200_masked_attention", g_masked.forward);
+  set("ditto_b200_masked_attention_backward", g_masked.backward);
+  set("ditto_b200_paged_workspace_bytes", g_masked.paged_bytes);
+  set("ditto_b200_paged_attention", g_masked.paged);
+  set("ditto_b200_cache_append", g_masked.append);
+  set("ditto_b200_cache_workspace_bytes", g_masked.cache_bytes);
+  set("ditto_b200_cache_fork", g_masked.fork);
+  set("ditto_b200_cache_free", g_masked.free);
+  set("ditto_b200_cache_compact", g_masked.compact);
+  Py_RETURN_NONE;
+}
+
 // A built module's compiled shape: plan(kind, batch, M, N, K, L, type code, heads, scale, act1, act2, bias1, bias2).
 struct Plan {
   int kind;                       // 0 softmax, 1 GEMM chain, 2 packed attention, 3 feed-forward
@@ -467,6 +895,14 @@ PyMethodDef kMethods[] = {DITTO_FAST("softmax", py_softmax),
                           DITTO_FAST("gemm", py_gemm),
                           DITTO_FAST("ffn", py_ffn),
                           DITTO_FAST("call", py_call),
+                          DITTO_FAST("masked", py_masked),
+                          DITTO_FAST("masked_backward", py_masked_backward),
+                          DITTO_FAST("paged", py_paged),
+                          DITTO_FAST("append", py_append),
+                          DITTO_FAST("cache_free", py_cache_free),
+                          DITTO_FAST("cache_fork", py_cache_fork),
+                          DITTO_FAST("cache_compact", py_cache_compact),
+                          {"bind_masked", py_bind_masked, METH_VARARGS, nullptr},
                           {"plan", py_plan, METH_VARARGS, nullptr},
                           {"bind", py_bind, METH_VARARGS, nullptr},
                           {"status", py_status, METH_VARARGS, nullptr},

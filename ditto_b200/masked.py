@@ -139,6 +139,7 @@ def _forward(query, key, value, out, want_lse, scale, causal, prefix, documents,
         rc = lib.ditto_b200_masked_attention(ctypes.byref(args), ws, need, _ops._status_ptr(query.device),
                                              torch.cuda.current_stream().cuda_stream)
     _lib.check(rc, "ditto_b200_masked_attention")
+    _ops._enable_fast(query.device)
     _ops.launch_count += 1
     return out, lse
 
@@ -158,6 +159,11 @@ def masked_attention(query, key, value, out=None, scale=1.0, causal=False, prefi
     float32 log of the sum of exponentials [batch, M, heads] (-inf for such a row; it gets no gradient).  Gradients of query, key and value
     flow where autograd asks for them (`out` cannot be given then).
     """
+    if _ops._fast is not None:
+        r = _ops._fast.masked(query, key, value, out, scale, causal, prefix, documents, slopes, cap, return_lse)
+        if r is not None:
+            _ops.launch_count += 1
+            return r
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (query, key, value)):
         if out is not None:
             raise ValueError("out cannot be given where gradients are asked for")
@@ -171,6 +177,11 @@ def masked_attention_backward(grad_out, query, key, value, out, lse, scale=1.0, 
                               cap=None):
     """Gradients (of query, key, value) of masked_attention from the gradient of its result; out and lse are what it returned for these
     operands and rules.  Sums are taken in a fixed order: the same call gives the same bits."""
+    if _ops._fast is not None:
+        r = _ops._fast.masked_backward(grad_out, query, key, value, out, lse, scale, causal, prefix, documents, slopes, cap)
+        if r is not None:
+            _ops.launch_count += 1
+            return r
     args = _masked_args(query, key, value, out, lse, scale, causal, prefix, documents, slopes, cap)
     _check(grad_out, "grad_out", query.dtype, query.device, 4, strided=True)
     if grad_out.shape != query.shape:
@@ -186,6 +197,7 @@ def masked_attention_backward(grad_out, query, key, value, out, lse, scale=1.0, 
             ctypes.byref(args), _ptr(grad_out), _strides(grad_out, _lib.Strides3), _ptr(dq), _ptr(dk), _ptr(dv), ws, need,
             _ops._status_ptr(query.device), torch.cuda.current_stream().cuda_stream)
     _lib.check(rc, "ditto_b200_masked_attention_backward")
+    _ops._enable_fast(query.device)
     _ops.launch_count += 1
     return dq, dk, dv
 
@@ -262,6 +274,11 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, query_s
     sequence's end may hold anything.  A page id out of range reads as zeros and shows in device_status(); lengths are cut to what a row of
     the table reaches.  The contents of block_table, lengths and query_starts are read on the device only: a captured call follows them.
     """
+    if _ops._fast is not None:
+        r = _ops._fast.paged(query, key_pages, value_pages, block_table, lengths, query_starts, out, scale, prefix, slopes, cap)
+        if r is not None:
+            _ops.launch_count += 1
+            return r
     dtype = _element(query)
     device = query.device
     _check(query, "query", dtype, device, 3, strided=True)
@@ -299,6 +316,7 @@ def paged_attention(query, key_pages, value_pages, block_table, lengths, query_s
         _buf, ws = _workspace(need, device)
         rc = lib.ditto_b200_paged_attention(ctypes.byref(args), ws, need, _ops._status_ptr(device), torch.cuda.current_stream().cuda_stream)
     _lib.check(rc, "ditto_b200_paged_attention")
+    _ops._enable_fast(query.device)
     _ops.launch_count += 1
     return out
 
@@ -308,6 +326,9 @@ def cache_append(keys, values, key_pages, value_pages, block_table, lengths, que
 
     Arguments as for paged_attention, which reads them from there: lengths counts the new tokens already.  Tokens whose place has no valid
     page are passed over, which shows in device_status()."""
+    if _ops._fast is not None and _ops._fast.append(keys, values, key_pages, value_pages, block_table, lengths, query_starts):
+        _ops.launch_count += 1
+        return
     dtype = _element(keys, "keys")
     device = keys.device
     _check(keys, "keys", dtype, device, 3, strided=True)
@@ -335,4 +356,5 @@ def cache_append(keys, values, key_pages, value_pages, block_table, lengths, que
     with _ops._on_device(device):
         rc = lib.ditto_b200_cache_append(ctypes.byref(args), _ops._status_ptr(device), torch.cuda.current_stream().cuda_stream)
     _lib.check(rc, "ditto_b200_cache_append")
+    _ops._enable_fast(keys.device)
     _ops.launch_count += 1

@@ -98,6 +98,8 @@ def _enable_fast(device):
         mod.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
             lib.ditto_b200_bmm_softmax_bmm, lib.ditto_b200_multi_head_attention, lib.ditto_b200_gemm_relu_gemm,
             lib.ditto_b200_ffn_ws, lib.ditto_b200_workspace_bytes)))
+        for name in _lib.MASKED_EXPORTS:
+            mod.bind_masked(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
         _fast = mod
     index = device.index if device.index is not None else torch.cuda.current_device()
     if index not in _fast_devices:
