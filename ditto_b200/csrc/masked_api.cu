@@ -80,7 +80,7 @@ int check_masked(const ditto_b200_masked_args* a) {
 }
 
 struct MaskedScratch {
-  size_t hulls, key_hulls;               // behind the blocks of keys
+  size_t mixed, key_blocks, hulls, key_hulls;      // of the documents, behind their runs
   size_t rows, norms, part, parts;       // of the backward pass
   size_t bytes;
 };
@@ -88,7 +88,9 @@ MaskedScratch masked_scratch(const ditto_b200_masked_args* a, bool backward, int
   MaskedScratch s = {};
   const size_t blocks = (a->L + 127) / 128, tile_tokens = 128 / (a->heads / a->kv_heads), tiles = (a->M + tile_tokens - 1) / tile_tokens;
   if (a->documents != nullptr) {
-    s.hulls = up256(a->batch * blocks * sizeof(masked::KeyBlock));
+    s.mixed = up256(static_cast<size_t>(a->batch) * a->L * sizeof(int2));
+    s.key_blocks = s.mixed + up256(a->batch * sizeof(int));
+    s.hulls = s.key_blocks + up256(a->batch * blocks * sizeof(masked::KeyBlock));
     s.key_hulls = s.hulls + up256(a->batch * tiles * sizeof(int2));
     s.bytes = s.key_hulls + (backward ? up256(a->batch * blocks * sizeof(int2)) : 0);
   }
@@ -100,6 +102,17 @@ MaskedScratch masked_scratch(const ditto_b200_masked_args* a, bool backward, int
     s.bytes = s.parts + up256(sms * sizeof(masked::KeyPartDesc));
   }
   return s;
+}
+
+// Launches the documents' plan of a call into its scratch memory and notes in p where what it finds is.
+cudaError_t plan_documents(masked::Params& p, const MaskedScratch& ws, uint8_t* base, bool backward, cudaStream_t stream) {
+  auto* runs = reinterpret_cast<int2*>(base);
+  auto* mixed = reinterpret_cast<int*>(base + ws.mixed);
+  auto* hulls = reinterpret_cast<int2*>(base + ws.hulls);
+  p.runs = runs, p.mixed = mixed, p.hulls = hulls;
+  return masked::launch_document_plan(p.documents, p.prefix, p.batch, p.M, p.L, p.causal, p.tile_tokens, p.tiles, runs, mixed,
+                                      reinterpret_cast<masked::KeyBlock*>(base + ws.key_blocks), hulls,
+                                      backward ? reinterpret_cast<int2*>(base + ws.key_hulls) : nullptr, stream);
 }
 
 // Query tiles of an item: two where that still leaves an item for every SM, so that each block of keys is loaded once for both.
@@ -234,12 +247,7 @@ int ditto_b200_masked_attention(const ditto_b200_masked_args* a, void* workspace
   p.status = status_word;
   if (a->documents != nullptr) {
     uint8_t* base = static_cast<uint8_t*>(workspace);
-    auto* key_blocks = reinterpret_cast<masked::KeyBlock*>(base);
-    auto* hulls = reinterpret_cast<int2*>(base + ws.hulls);
-    p.key_blocks = key_blocks;
-    p.hulls = hulls;
-    const cudaError_t e = masked::launch_document_plan(a->documents, a->prefix, p.batch, p.M, p.L, p.causal, p.tile_tokens, p.tiles, key_blocks,
-                                                       hulls, nullptr, st);
+    const cudaError_t e = plan_documents(p, ws, base, false, st);
     if (e != cudaSuccess) return cuda_fail("masked_attention plan", e);
   }
   const cudaError_t e = masked::launch_forward_any(p, p.d <= 64 ? 64 : 128, a->dtype == DITTO_DTYPE_BF16, false, nt,
@@ -300,11 +308,9 @@ int ditto_b200_masked_attention_backward(const ditto_b200_masked_args* a, const 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (a->documents != nullptr) {
-    auto* key_blocks = reinterpret_cast<masked::KeyBlock*>(base);
-    auto* hulls = reinterpret_cast<int2*>(base + ws.hulls);
-    auto* key_hulls = reinterpret_cast<int2*>(base + ws.key_hulls);
-    p.key_blocks = key_blocks, p.hulls = hulls, p.key_hulls = key_hulls;
-    e = masked::launch_document_plan(a->documents, a->prefix, p.batch, p.M, p.L, p.causal, p.tile_tokens, p.tiles, key_blocks, hulls, key_hulls, st);
+    e = plan_documents(f, ws, base, true, st);
+    p.runs = f.runs, p.mixed = f.mixed, p.hulls = f.hulls;
+    p.key_hulls = reinterpret_cast<int2*>(base + ws.key_hulls);
   }
   if (e == cudaSuccess) {
     if (p.d <= 64)

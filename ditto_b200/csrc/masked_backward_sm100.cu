@@ -15,6 +15,7 @@
 // fp16: P is taken times 2^14 and dS times a power of two from the largest row norms of dO and V, so that neither leaves the type's range
 // nor falls below its normal numbers as weights of a few thousand keys would.
 #include <atomic>
+#include <climits>
 
 #include "host_util.cuh"
 #include "masked_backward_sm100.cuh"
@@ -408,10 +409,19 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
       const KeySegment& s = segments[slot];
       if (!s.valid) break;
       const int lo = s.lo, hi = s.hi, key = s.block * kKeys + row;
-      int doc = -2;
-      if (GENERAL && p.documents != nullptr && key < p.L) doc = p.documents[static_cast<size_t>(s.seq) * p.L + key];
-      // first column that sees the key: causal, and not in the prefix that all see
-      const bool bounded = p.causal && !(key < s.prefix);
+      // positions that see the key: from `first` up to `end` (causal, and not in the prefix that all see; documents)
+      int first = p.causal && !(key < s.prefix) ? key : INT_MIN / 256, end = INT_MAX / 256, doc = -2;
+      bool mixed = false;
+      if (p.documents != nullptr) {
+        if (key < p.L) {
+          const size_t at = static_cast<size_t>(s.seq) * p.L + key;
+          const int2 run = p.runs[at];
+          first = max(first, run.x);
+          end = run.y;
+          doc = p.documents[at];
+        }
+        mixed = p.mixed[s.seq] != 0;
+      }
       for (int i = lo; i < hi; ++i, ++n) {
         const int st = n & 1;
         const TileRows& rows = *reinterpret_cast<const TileRows*>(smem + LO::kOffRows + st * sizeof(TileRows));
@@ -419,8 +429,10 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&bar->s_full, n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
-        const int from = bounded ? (key - (p.L - p.M) - i * p.tile_tokens) * p.group - half * 64 : 0;      // columns in front of it do not
-        const bool cut = __any_sync(0xffffffffu, from > 0);
+        const int pos0 = p.L - p.M + i * p.tile_tokens;      // of column 0; columns from .. to - 1 of this half see the key
+        const int from = first > pos0 ? min(first - pos0, kRows) * p.group - half * 64 : 0;
+        const int to = min(max(end - pos0, 0), kRows) * p.group - half * 64;
+        const bool cut = __any_sync(0xffffffffu, from > 0), cut_end = __any_sync(0xffffffffu, to < 64);
         float w[64];
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
@@ -451,7 +463,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
                 sv[u + 3] = __float_as_uint(fmaf(__uint_as_float(sv[u + 3]), sc, -sl.w * fabsf(ps.w - at)));
               }
             }
-            if (p.documents != nullptr) {
+          }
+          if (mixed) {
 #pragma unroll
               for (int u = 0; u < 32; u += 4) {
                 const int4 d = *reinterpret_cast<const int4*>(&rows.doc[half * 64 + ch * 32 + u]);
@@ -460,12 +473,16 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
                 if (d.z != doc) sv[u + 2] = __float_as_uint(-INFINITY);
                 if (d.w != doc) sv[u + 3] = __float_as_uint(-INFINITY);
               }
-            }
           }
           if (cut) {
 #pragma unroll
             for (int u = 0; u < 32; ++u)
               if (ch * 32 + u < from) sv[u] = __float_as_uint(-INFINITY);
+          }
+          if (cut_end) {
+#pragma unroll
+            for (int u = 0; u < 32; ++u)
+              if (ch * 32 + u >= to) sv[u] = __float_as_uint(-INFINITY);
           }
           const uint64_t c2 = pack_f32x2(c, c);
 #pragma unroll
@@ -783,15 +800,25 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       const bool valid = r_token < p.tile_tokens && token < s.tokens;
       const TileRows& rows = p.rows[(static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + s.first_token / p.tile_tokens];
       const float off = p_log2 - rows.lse[row], delta = rows.delta[row], slope = GENERAL ? rows.slope[row] : 0.f;
-      const int doc = GENERAL ? rows.doc[row] : 0;
-      const int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0;
+      int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0, low = 0, doc = -1;
+      bool mixed = false;
+      if (p.documents != nullptr) {
+        if (valid) {
+          const size_t at = static_cast<size_t>(s.seq) * p.L + pos;
+          const int2 run = p.runs[at];
+          low = run.x;
+          limit = min(limit, run.y);
+          doc = p.documents[at];
+        }
+        mixed = p.mixed[s.seq] != 0;
+      }
       for (int j = lo; j < hi; ++j, ++n) {
         const int st = n & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full, n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
         const int k0 = j * kKeys + half * 64;
-        const bool cut = __any_sync(0xffffffffu, limit < k0 + 64);
+        const bool cut = __any_sync(0xffffffffu, limit < k0 + 64), cut_low = __any_sync(0xffffffffu, low > k0);
         float w[64];
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
@@ -816,17 +843,19 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
               for (int u = 0; u < 32; ++u)
                 sv[u] = __float_as_uint(fmaf(__uint_as_float(sv[u]), sc, -slope * fabsf(far - static_cast<float>(u))));
             }
-            if (p.documents != nullptr) {
-              const int only = p.key_blocks[static_cast<size_t>(s.seq) * p.blocks + j].only;
-              if (__any_sync(0xffffffffu, doc >= 0 && doc != only)) {
-                const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
+          }
+          if (mixed) {
+            const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
 #pragma unroll
-                for (int u = 0; u < 32; ++u) {
-                  if (ids[min(k0 + ch * 32 + u, p.L - 1)] != doc) sv[u] = __float_as_uint(-INFINITY);
-                  if (u % 8 == 7) asm volatile("" ::: "memory");       // (eight ids at a time: registers)
-                }
-              }
+            for (int u = 0; u < 32; ++u) {
+              if (ids[min(k0 + ch * 32 + u, p.L - 1)] != doc) sv[u] = __float_as_uint(-INFINITY);
+              if (u % 8 == 7) asm volatile("" ::: "memory");       // (eight ids at a time: registers)
             }
+          }
+          if (cut_low) {
+#pragma unroll
+            for (int u = 0; u < 32; ++u)
+              if (u < low - k0 - ch * 32) sv[u] = __float_as_uint(-INFINITY);
           }
           if (cut) {
             const int lim = limit - k0 - ch * 32;
@@ -962,7 +991,7 @@ cudaError_t launch_backward(const BackwardParams& p, int sms, cudaStream_t strea
   cudaLaunchAttribute attr[1];
   const cudaError_t e = launch_kernel(config(ctas < 8 * sms ? ctas : 8 * sms, kRowThreads, 0, stream, attr), backward_rows_kernel<BF16>, p);
   if (e != cudaSuccess) return e;
-  const bool general = p.cap_out != 0.f || p.slopes != nullptr || p.documents != nullptr;
+  const bool general = p.cap_out != 0.f || p.slopes != nullptr;
   return general ? launch_products<D, BF16, true>(p, sms, stream) : launch_products<D, BF16, false>(p, sms, stream);
 }
 

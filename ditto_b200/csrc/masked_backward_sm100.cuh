@@ -38,7 +38,8 @@ struct BackwardParams {
   const float* slopes;
   const int* prefix;
   const int* documents;
-  const KeyBlock* key_blocks; // with documents
+  const int2* runs;           // with documents, as in the forward pass
+  const int* mixed;
   const int2* hulls;          // [batch][tiles]
   const int2* key_hulls;      // [batch][blocks]
   float* part;                // [CTA][2][dK, dV][128][D]

@@ -394,11 +394,19 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       const int token = s.first_token + t * p.tile_tokens + r_token, pos = token + s.keys - s.tokens;
       const bool valid = row_used && token < s.tokens;
       const int head = s.kv_head * p.group + r_head;
-      int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0, doc = -1;
+      // the row sees keys from low up to limit; documents in another order than rising: those of them that have its id
+      int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0, low = 0, doc = -1;
+      bool mixed = false;
       if constexpr (!PAGED) {
         if (p.documents != nullptr) {
-          if (valid) doc = p.documents[static_cast<size_t>(s.seq) * p.L + pos];
-          if (doc < 0) limit = 0;
+          if (valid) {
+            const size_t at = static_cast<size_t>(s.seq) * p.L + pos;
+            const int2 run = p.runs[at];
+            low = run.x;
+            limit = min(limit, run.y);
+            doc = p.documents[at];
+          }
+          mixed = p.mixed[s.seq] != 0;
         }
       }
       const float slope = p.slopes != nullptr && valid ? p.slopes[head] * 1.4426950408889634f : 0.f;
@@ -431,8 +439,12 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         }
         if constexpr (!PAGED) {
           if (p.documents != nullptr) {
-            const int only = p.key_blocks[static_cast<size_t>(s.seq) * ((p.L + kKeys - 1) / kKeys) + j].only;
-            if (__any_sync(0xffffffffu, doc >= 0 && doc != only)) {
+            if (__any_sync(0xffffffffu, low > k0)) {
+#pragma unroll
+              for (int i = 0; i < kKeys; ++i)
+                if (i < low - k0) sv[i] = __float_as_uint(-INFINITY);
+            }
+            if (mixed) {
               const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
 #pragma unroll
               for (int i = 0; i < kKeys; ++i) {

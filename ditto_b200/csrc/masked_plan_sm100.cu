@@ -21,11 +21,35 @@ __device__ __forceinline__ int warp_min(int v) {
 }
 __device__ __forceinline__ int warp_max(int v) { return -warp_min(-v); }
 
+// Maximum over the threads up to this one; *before: of those in front of it (`none` for the first), *all: of all.
+__device__ __forceinline__ int block_max(int v, int none, int* scratch, int* before, int* all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl = max(incl, x);
+  }
+  const int left = __shfl_up_sync(0xffffffffu, incl, 1);
+  __syncthreads();
+  if (lane == 31) scratch[warp] = incl;
+  __syncthreads();
+  int front = none, whole = none;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) front = max(front, scratch[w]);
+    whole = max(whole, scratch[w]);
+  }
+  *before = lane == 0 ? front : max(front, left);
+  *all = whole;
+  return max(front, incl);
+}
+
 // One CTA a batch row.  Document ids may come in any order: a block is skipped where the ranges of ids of its keys and of a tile's queries
 // do not meet, which for documents that follow one another are the blocks that hold none of the tile's, and never one that does.
 __global__ void __launch_bounds__(kPlanThreads, 1) document_plan_kernel(const int* documents, const int* prefix, int M, int L, int causal,
-                                                                        int tile_tokens, int tiles, KeyBlock* key_blocks, int2* hulls,
-                                                                        int2* key_hulls) {
+                                                                        int tile_tokens, int tiles, int2* runs, int* mixed,
+                                                                        KeyBlock* key_blocks, int2* hulls, int2* key_hulls) {
+  __shared__ int scratch[kPlanThreads / 32];
   grid_dependency_wait();
   grid_launch_dependents();
   const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = kPlanThreads / 32;
@@ -33,20 +57,45 @@ __global__ void __launch_bounds__(kPlanThreads, 1) document_plan_kernel(const in
   const int* ids = documents + static_cast<size_t>(b) * L;
   KeyBlock* mine = key_blocks + static_cast<size_t>(b) * blocks;
   const int pre = prefix != nullptr ? prefix[b] : 0;
+  // Runs of equal ids: a position's run begins at the last change of id up to it and ends at the first one behind it.  They are its document
+  // where every id has one run, which is certain where the ids rise.
+  int2* my_runs = runs + static_cast<size_t>(b) * L;
+  int begin = 0, highest = -1;
+  bool falls = false;
+  for (int base = 0; base < L; base += kPlanThreads) {
+    const int k = base + static_cast<int>(threadIdx.x), id = k < L ? ids[k] : -1;
+    const bool change = k < L && (k == 0 || ids[k - 1] != id);
+    int before, all;
+    const int at = max(begin, block_max(change ? k : 0, 0, scratch, &before, &all));
+    begin = max(begin, all);
+    block_max(id, -1, scratch, &before, &all);
+    falls |= change && id >= 0 && id <= max(highest, before);
+    highest = max(highest, all);
+    if (k < L) my_runs[k].x = at;
+  }
+  const bool any_order = __syncthreads_or(falls);
+  if (threadIdx.x == 0) mixed[b] = any_order;
+  int end = 0;                                         // (of the positions counted from the row's end)
+  for (int base = 0; base < L; base += kPlanThreads) {
+    const int r = base + static_cast<int>(threadIdx.x), k = L - 1 - r, id = r < L ? ids[k] : -1;
+    const bool change = r < L && (r == 0 || ids[k + 1] != id);
+    int before, all;
+    const int at = max(end, block_max(change ? r : 0, 0, scratch, &before, &all));
+    end = max(end, all);
+    if (r < L) my_runs[k] = id < 0 ? make_int2(0, 0) : any_order ? make_int2(0, L) : make_int2(my_runs[k].x, L - at);
+  }
   for (int j = warp; j < blocks; j += warps) {
-    int least = INT_MAX, most = -1, low = INT_MAX, high = INT_MIN;
+    int least = INT_MAX, most = -1;
 #pragma unroll
     for (int u = 0; u < kKeys / 32; ++u) {
       const int k = j * kKeys + u * 32 + lane;
       if (k < L) {
         const int id = ids[k];
-        low = min(low, id);
-        high = max(high, id);
         if (id >= 0) least = min(least, id), most = max(most, id);
       }
     }
-    least = warp_min(least), most = warp_max(most), low = warp_min(low), high = warp_max(high);
-    if (lane == 0) mine[j] = {least, most, low == high && low >= 0 ? low : -1, 0};
+    least = warp_min(least), most = warp_max(most);
+    if (lane == 0) mine[j] = {least, most};
   }
   __syncthreads();
   for (int tile = warp; tile < tiles; tile += warps) {
@@ -147,10 +196,11 @@ cudaLaunchConfig_t config(int grid, int threads, cudaStream_t stream, cudaLaunch
 }  // namespace
 
 cudaError_t launch_document_plan(const int* documents, const int* prefix, int batch, int M, int L, int causal, int tile_tokens, int tiles,
-                                 KeyBlock* key_blocks, int2* hulls, int2* key_hulls, cudaStream_t stream) {
+                                 int2* runs, int* mixed, KeyBlock* key_blocks, int2* hulls, int2* key_hulls, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = config(batch, kPlanThreads, stream, attr);
-  return launch_kernel(cfg, document_plan_kernel, documents, prefix, M, L, causal, tile_tokens, tiles, key_blocks, hulls, key_hulls);
+  return launch_kernel(cfg, document_plan_kernel, documents, prefix, M, L, causal, tile_tokens, tiles, runs, mixed, key_blocks, hulls,
+                       key_hulls);
 }
 
 cudaError_t launch_sum_parts(const Params& p, int d, bool bf16, int tiles, int grid, cudaStream_t stream) {

@@ -16,10 +16,9 @@ namespace masked {
 constexpr int kRows = 128;        // rows of a query tile
 constexpr int kKeys = 128;        // keys of a block
 
-// Documents of a block of 128 keys: smallest and largest id that is not negative (an empty range where there is none), and the id
-// that all of them have, else -1.
+// Documents of a block of 128 keys: smallest and largest id that is not negative (an empty range where there is none).
 struct KeyBlock {
-  int least, most, only, unused;
+  int least, most;
 };
 
 // An item that a CTA begins and does not end (split over several CTAs): what the combining kernel needs to find its parts.
@@ -45,7 +44,8 @@ struct Params {
   const float* slopes;        // [heads] or null
   const int* prefix;          // [batch] or null
   const int* documents;       // [batch, L] or null
-  const KeyBlock* key_blocks; // [batch, blocks of 128 keys], with documents
+  const int2* runs;           // [batch, L]: where the position's document begins and ends; (0, 0) of a negative one
+  const int* mixed;           // [batch]: 1 where ids come in another order than rising, so that runs say nothing and ids are compared
   const int2* hulls;          // [batch, tiles]: first block and the one behind the last that the tile's documents reach
   // paged
   const int* table;
