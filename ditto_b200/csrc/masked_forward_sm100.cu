@@ -275,6 +275,12 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       tc_fence_after_sync();
       return r;
     };
+    // (of two barriers at once: a vote and a fence less)
+    auto wait_both = [&](uint64_t* b, uint32_t parity, uint64_t* b2, uint32_t parity2, uint32_t code) {
+      const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code) && mbar_wait(b2, parity2, abort_word, code));
+      tc_fence_after_sync();
+      return r;
+    };
     auto wait_kv = [&](int n) { return wait(&bar->kv_full[n % kStages], (n / kStages) & 1, 0x310); };      // n: 2 block, or 2 block + 1
     auto issue_s = [&](int block) {
       const int st = (2 * block) % kStages;
@@ -339,22 +345,30 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       }
       for (int j = first; j < last; j += kStep, ++n) {
         const int next = j + kStep, nv = 2 * (block0 + j) + 1, sv = nv % kStages;
-        if (!(ok = wait_kv(nv))) break;
+        // What is most likely there is waited for first.  With one tile the next keys are waited for behind P V: they may still be on
+        // their way where memory is the bound, and the values' place in the ring is wanted back.
+        if (NT == 2 && next < last) {
+          const int nk = 2 * (block0 + next);
+          if (!(ok = wait_both(&bar->kv_full[sv], (nv / kStages) & 1, &bar->kv_full[nk % kStages], (nk / kStages) & 1, 0x310))) break;
+        } else {
+          if (!(ok = wait_kv(nv))) break;
+        }
         if (j == first) {                              // a new accumulator: what it held has been read
           if (!(ok = wait(&bar->o_free[buf], (uses_o & 1) ^ 1, 0x320))) break;      // (at once the first time)
           ++uses_o;
         }
         const uint64_t db = dv0 + ((sv * kTile) >> 4);
-        if (!(ok = wait(&bar->p_part[buf][0], n & 1, 0x340) && take_turn())) break;
+        if (!(ok = wait_both(&bar->turn[buf], (turns & 1) ^ (buf == 0 ? 1u : 0u), &bar->p_part[buf][0], n & 1, 0x340))) break;
+        ++turns;
 #pragma unroll
         for (int i = 0; i < kSplit / 16; ++i)
           umma_ts_elected(d_o, d_s + i * 8, db + ((i * 2048) >> 4), idesc_o, i > 0 || j > first ? 1u : 0u, issuer);
-        if (next < last && !(ok = wait_kv(2 * (block0 + next)))) break;
         if (!(ok = wait(&bar->p_part[buf][1], n & 1, 0x341))) break;
 #pragma unroll
         for (int i = kSplit / 16; i < kKeys / 16; ++i) umma_ts_elected(d_o, d_s + i * 8, db + ((i * 2048) >> 4), idesc_o, 1u, issuer);
         umma_commit_elected(&bar->kv_empty[sv], issuer);
         if (next < last) {
+          if (NT == 1 && !(ok = wait_kv(2 * (block0 + next)))) break;
           issue_s(block0 + next);
           if (next + kStep >= last) umma_commit_elected(&bar->q_empty[t], issuer);
         } else {
@@ -410,6 +424,9 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         }
       }
       const float slope = p.slopes != nullptr && valid ? p.slopes[head] * 1.4426950408889634f : 0.f;
+      // the first block that a row of this warp does not see whole, and the last one in which one does not see the first key (documents)
+      const int cut = __reduce_min_sync(0xffffffffu, limit) / kKeys, cut_low = __reduce_max_sync(0xffffffffu, low);
+      const bool modified = p.cap_out != 0.f || p.slopes != nullptr || mixed;
       RowReference ref(c);
       if (limit == 0) ref.m = 0.f, ref.large = false;      // sees nothing: asks for no rescale
       float l = 0.f;
@@ -421,29 +438,18 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         uint32_t sv[kKeys];
         tmem_ld_x128_wait(s_col, sv);
         const int k0 = j * kKeys;
-        if (p.cap_out != 0.f) {
+        if (modified) {
+          if (p.cap_out != 0.f) {
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) sv[i] = __float_as_uint(p.cap_out * tanh_of(__uint_as_float(sv[i]) * p.cap_in));
-        }
-        if (p.slopes != nullptr) {
-          const float f = p.cap_out != 0.f ? 1.0f : p.score_log2, far = static_cast<float>(pos - k0);
+            for (int i = 0; i < kKeys; ++i) sv[i] = __float_as_uint(p.cap_out * tanh_of(__uint_as_float(sv[i]) * p.cap_in));
+          }
+          if (p.slopes != nullptr) {
+            const float f = p.cap_out != 0.f ? 1.0f : p.score_log2, far = static_cast<float>(pos - k0);
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            sv[i] = __float_as_uint(fmaf(__uint_as_float(sv[i]), f, -slope * fabsf(far - static_cast<float>(i))));
-        }
-        if (__any_sync(0xffffffffu, limit < k0 + kKeys)) {
-          const int lim = limit - k0;
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            if (i >= lim) sv[i] = __float_as_uint(-INFINITY);
-        }
-        if constexpr (!PAGED) {
-          if (p.documents != nullptr) {
-            if (__any_sync(0xffffffffu, low > k0)) {
-#pragma unroll
-              for (int i = 0; i < kKeys; ++i)
-                if (i < low - k0) sv[i] = __float_as_uint(-INFINITY);
-            }
+            for (int i = 0; i < kKeys; ++i)
+              sv[i] = __float_as_uint(fmaf(__uint_as_float(sv[i]), f, -slope * fabsf(far - static_cast<float>(i))));
+          }
+          if constexpr (!PAGED) {
             if (mixed) {
               const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
 #pragma unroll
@@ -453,6 +459,17 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
               }
             }
           }
+        }
+        if (j >= cut) {
+          const int lim = limit - k0;
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (i >= lim) sv[i] = __float_as_uint(-INFINITY);
+        }
+        if (!PAGED && cut_low > k0) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (i < low - k0) sv[i] = __float_as_uint(-INFINITY);
         }
         float mx[8];
 #pragma unroll
