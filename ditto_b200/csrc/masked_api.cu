@@ -56,7 +56,7 @@ int set_rules(masked::Params& p, float scale, float cap, const float* slopes, co
   p.slopes = slopes;
   p.prefix = prefix;
   p.score_log2 = scale * kLog2e;
-  p.cap_in = cap > 0.f ? 2.0f * scale * kLog2e / cap : 0.f;
+  p.cap_in = cap > 0.f ? scale / cap : 0.f;
   p.cap_out = cap > 0.f ? cap * kLog2e : 0.f;
   p.c = cap > 0.f || slopes != nullptr ? 1.0f : p.score_log2;
   return DITTO_OK;

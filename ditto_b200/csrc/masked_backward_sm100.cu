@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid
       t.lse[r] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
       t.delta[r] = dot;
       t.doc[r] = p.documents != nullptr && valid ? p.documents[static_cast<size_t>(b) * p.L + pos] : -1;
-      t.slope[r] = p.slopes != nullptr && valid ? p.slopes[head] * 1.4426950408889634f : 0.f;
+      t.slope[r] = p.slopes != nullptr && valid ? p.slopes[head] * -1.4426950408889634f : 0.f;
       t.pos[r] = static_cast<float>(pos);
     }
   }
@@ -438,29 +438,39 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         for (int ch = 0; ch < 2; ++ch) {
           uint32_t sv[32];
           tmem_ld_x32_wait(s_col + ch * 32, sv);
-          float g[32];
+          // (w holds what dS is the product of with dP - delta: first 1 - tanh^2, then that times the weight)
           if constexpr (GENERAL) {
             if (p.cap_out != 0.f) {
+              capped(sv, p.cap_in, 1.0f);
+              const uint64_t one2 = pack_f32x2(1.0f, 1.0f), out2 = pack_f32x2(p.cap_out, p.cap_out);
 #pragma unroll
-              for (int u = 0; u < 32; ++u) {
-                const float t = tanh_of(__uint_as_float(sv[u]) * p.cap_in);
-                sv[u] = __float_as_uint(p.cap_out * t);
-                g[u] = fmaf(-t, t, 1.0f);
+              for (int u = 0; u < 32; u += 2) {
+                const uint64_t t = pack_f32x2(__uint_as_float(sv[u]), __uint_as_float(sv[u + 1]));
+                unpack_f32x2(fma_f32x2(mul_f32x2(t, pack_f32x2(-1.0f, -1.0f)), t, one2), w[ch * 32 + u], w[ch * 32 + u + 1]);
+                float y0, y1;
+                unpack_f32x2(mul_f32x2(t, out2), y0, y1);
+                sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
             } else {
 #pragma unroll
-              for (int u = 0; u < 32; ++u) g[u] = 1.0f;
+              for (int u = 0; u < 32; ++u) w[ch * 32 + u] = 1.0f;
             }
             if (p.slopes != nullptr) {
               const float sc = p.cap_out != 0.f ? 1.0f : p.score_log2, at = static_cast<float>(key);
+              const uint64_t sc2 = pack_f32x2(sc, sc), at2 = pack_f32x2(-at, -at);
 #pragma unroll
               for (int u = 0; u < 32; u += 4) {
                 const float4 sl = *reinterpret_cast<const float4*>(&rows.slope[half * 64 + ch * 32 + u]);
                 const float4 ps = *reinterpret_cast<const float4*>(&rows.pos[half * 64 + ch * 32 + u]);
-                sv[u] = __float_as_uint(fmaf(__uint_as_float(sv[u]), sc, -sl.x * fabsf(ps.x - at)));
-                sv[u + 1] = __float_as_uint(fmaf(__uint_as_float(sv[u + 1]), sc, -sl.y * fabsf(ps.y - at)));
-                sv[u + 2] = __float_as_uint(fmaf(__uint_as_float(sv[u + 2]), sc, -sl.z * fabsf(ps.z - at)));
-                sv[u + 3] = __float_as_uint(fmaf(__uint_as_float(sv[u + 3]), sc, -sl.w * fabsf(ps.w - at)));
+#pragma unroll
+                for (int q = 0; q < 4; q += 2) {
+                  float d0, d1;
+                  unpack_f32x2(add_f32x2(q == 0 ? pack_f32x2(ps.x, ps.y) : pack_f32x2(ps.z, ps.w), at2), d0, d1);
+                  const uint64_t bias = mul_f32x2(q == 0 ? pack_f32x2(sl.x, sl.y) : pack_f32x2(sl.z, sl.w), pack_f32x2(fabsf(d0), fabsf(d1)));
+                  float y0, y1;
+                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sv[u + q]), __uint_as_float(sv[u + q + 1])), sc2, bias), y0, y1);
+                  sv[u + q] = __float_as_uint(y0), sv[u + q + 1] = __float_as_uint(y1);
+                }
               }
             }
           }
@@ -498,8 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
               pk[v] = pack2<BF16>(p0, p1);
               pk[v + 1] = pack2<BF16>(p2, p3);
               const int x = ch * 32 + u;
-              w[x] = GENERAL ? p0 * g[u] : p0, w[x + 1] = GENERAL ? p1 * g[u + 1] : p1;
-              w[x + 2] = GENERAL ? p2 * g[u + 2] : p2, w[x + 3] = GENERAL ? p3 * g[u + 3] : p3;
+              w[x] = GENERAL ? p0 * w[x] : p0, w[x + 1] = GENERAL ? p1 * w[x + 1] : p1;
+              w[x + 2] = GENERAL ? p2 * w[x + 2] : p2, w[x + 3] = GENERAL ? p3 * w[x + 3] : p3;
             }
             // (packed weights go over the first half of this half's own columns)
             tmem_st_x8(s_col + ch * 16 + q * 8, pk);
@@ -812,6 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         }
         mixed = p.mixed[s.seq] != 0;
       }
+      const bool behind = p.causal && s.prefix <= s.keys - s.tokens + s.first_token + 1;      // every key that a row sees is at or in front of it
       for (int j = lo; j < hi; ++j, ++n) {
         const int st = n & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full, n & 1, abort_word, 0x800));
@@ -824,25 +835,23 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         for (int ch = 0; ch < 2; ++ch) {
           uint32_t sv[32];
           tmem_ld_x32_wait(lane_base + kColS + half * 64 + ch * 32, sv);
-          float g[32];
           if constexpr (GENERAL) {
             if (p.cap_out != 0.f) {
+              capped(sv, p.cap_in, 1.0f);
+              const uint64_t one2 = pack_f32x2(1.0f, 1.0f), out2 = pack_f32x2(p.cap_out, p.cap_out);
 #pragma unroll
-              for (int u = 0; u < 32; ++u) {
-                const float t = tanh_of(__uint_as_float(sv[u]) * p.cap_in);
-                sv[u] = __float_as_uint(p.cap_out * t);
-                g[u] = fmaf(-t, t, 1.0f);
+              for (int u = 0; u < 32; u += 2) {
+                const uint64_t t = pack_f32x2(__uint_as_float(sv[u]), __uint_as_float(sv[u + 1]));
+                unpack_f32x2(fma_f32x2(mul_f32x2(t, pack_f32x2(-1.0f, -1.0f)), t, one2), w[ch * 32 + u], w[ch * 32 + u + 1]);
+                float y0, y1;
+                unpack_f32x2(mul_f32x2(t, out2), y0, y1);
+                sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
             } else {
 #pragma unroll
-              for (int u = 0; u < 32; ++u) g[u] = 1.0f;
+              for (int u = 0; u < 32; ++u) w[ch * 32 + u] = 1.0f;
             }
-            if (p.slopes != nullptr) {
-              const float sc = p.cap_out != 0.f ? 1.0f : p.score_log2, far = static_cast<float>(pos - k0 - ch * 32);
-#pragma unroll
-              for (int u = 0; u < 32; ++u)
-                sv[u] = __float_as_uint(fmaf(__uint_as_float(sv[u]), sc, -slope * fabsf(far - static_cast<float>(u))));
-            }
+            if (p.slopes != nullptr) biased(sv, p.cap_out != 0.f ? 1.0f : p.score_log2, -slope, static_cast<float>(pos - k0 - ch * 32), behind);
           }
           if (mixed) {
             const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
@@ -868,8 +877,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
           for (int u = 0; u < 32; u += 2) {
             float p0, p1;
             unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, off2, weights_on_fma(u / 2)), p0, p1);
-            w[ch * 32 + u] = GENERAL ? p0 * g[u] : p0;
-            w[ch * 32 + u + 1] = GENERAL ? p1 * g[u + 1] : p1;
+            w[ch * 32 + u] = GENERAL ? p0 * w[ch * 32 + u] : p0;
+            w[ch * 32 + u + 1] = GENERAL ? p1 * w[ch * 32 + u + 1] : p1;
           }
         }
         tc_fence_before_sync();

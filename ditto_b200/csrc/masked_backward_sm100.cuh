@@ -11,7 +11,7 @@ struct TileRows {
   float lse[kRows];      // log2 of the sum of exponentials
   float delta[kRows];    // sum over d of grad_out times out
   int doc[kRows];
-  float slope[kRows];    // slopes[head] log2(e)
+  float slope[kRows];    // -slopes[head] log2(e)
   float pos[kRows];      // position of the row's query
 };
 static_assert(sizeof(TileRows) == 2560, "a bulk copy of whole 16-byte pieces");

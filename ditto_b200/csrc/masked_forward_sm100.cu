@@ -427,6 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       // the first block that a row of this warp does not see whole, and the last one in which one does not see the first key (documents)
       const int cut = __reduce_min_sync(0xffffffffu, limit) / kKeys, cut_low = __reduce_max_sync(0xffffffffu, low);
       const bool modified = p.cap_out != 0.f || p.slopes != nullptr || mixed;
+      // every key that a row sees is at or in front of it
+      const bool behind = p.causal && s.prefix <= s.keys - s.tokens + s.first_token + t * p.tile_tokens + 1;
       RowReference ref(c);
       if (limit == 0) ref.m = 0.f, ref.large = false;      // sees nothing: asks for no rescale
       float l = 0.f;
@@ -439,16 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         tmem_ld_x128_wait(s_col, sv);
         const int k0 = j * kKeys;
         if (modified) {
-          if (p.cap_out != 0.f) {
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i) sv[i] = __float_as_uint(p.cap_out * tanh_of(__uint_as_float(sv[i]) * p.cap_in));
-          }
-          if (p.slopes != nullptr) {
-            const float f = p.cap_out != 0.f ? 1.0f : p.score_log2, far = static_cast<float>(pos - k0);
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-              sv[i] = __float_as_uint(fmaf(__uint_as_float(sv[i]), f, -slope * fabsf(far - static_cast<float>(i))));
-          }
+          if (p.cap_out != 0.f) capped(sv, p.cap_in, p.cap_out);
+          if (p.slopes != nullptr) biased(sv, p.cap_out != 0.f ? 1.0f : p.score_log2, slope, static_cast<float>(pos - k0), behind);
           if constexpr (!PAGED) {
             if (mixed) {
               const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;

@@ -39,7 +39,7 @@ struct Params {
   int items;                  // batch x kv heads x groups of tiles (dense)
   int causal;
   float c;                    // factor of a score in the exponent of 2: scale log2(e), or 1 where cap or bias have applied it
-  float cap_in, cap_out;      // 2 scale log2(e) / cap, and cap log2(e); cap_out 0: no cap
+  float cap_in, cap_out;      // scale / cap, and cap log2(e); cap_out 0: no cap
   float score_log2;           // scale log2(e)
   const float* slopes;        // [heads] or null
   const int* prefix;          // [batch] or null
@@ -224,17 +224,70 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// tanh(x) from y = 2 x log2(e): 1 - 2 / (1 + 2^y), to about 1.5e-7 absolute.
-__device__ __forceinline__ float tanh_of(float y) {
+// tanh(x) = 1 - 2 / (1 + e^2x), to about 1.5e-7 absolute.
+__device__ __forceinline__ float tanh_of(float x) {
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 2.8853900817779268f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return fmaf(-2.0f, r, 1.0f);
 }
 
-}  // namespace masked
+// s <- f tanh(k s) for a thread's scores; the whole warp together.  Scores that are small beside the cap, the usual ones, take
+// tanh(x) = x q(x^2) on the multiply-add pipe: |x| <= 3/4, q of degree 5, least maximum relative error (iteratively reweighted least squares)
+// 2.9e-8.  tanh_of has two instructions of the special-function unit in it, which the exponentials behind keep busy already: with it alone
+// the forward pass of 16 heads of 8192 x 8192 x 128, causal, took 529 us instead of 317.
+template <int N>
+__device__ __forceinline__ void capped(uint32_t (&s)[N], float k, float f) {
+  const uint64_t k2 = pack_f32x2(k, k);
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t x = mul_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), k2);
+    float x0, x1;
+    unpack_f32x2(x, x0, x1);
+    s[i] = __float_as_uint(x0), s[i + 1] = __float_as_uint(x1);
+    most = max3(most, fabsf(x0), fabsf(x1));
+  }
+  if (__all_sync(0xffffffffu, most <= 0.75f)) {
+    auto both = [&](float c) { return pack_f32x2(f * c, f * c); };
+    const uint64_t c0 = both(1.0f), c1 = both(-0x1.5554a4p-2f), c2 = both(0x1.10ed66p-3f), c3 = both(-0x1.b5604ep-5f), c4 = both(0x1.423392p-6f),
+                   c5 = both(-0x1.389a58p-8f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t x = pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), z = mul_f32x2(x, x);
+      uint64_t q = fma_f32x2(c5, z, c4);
+      q = fma_f32x2(q, z, c3);
+      q = fma_f32x2(q, z, c2);
+      q = fma_f32x2(q, z, c1);
+      q = fma_f32x2(q, z, c0);
+      float y0, y1;
+      unpack_f32x2(mul_f32x2(x, q), y0, y1);
+      s[i] = __float_as_uint(y0), s[i + 1] = __float_as_uint(y1);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = __float_as_uint(f * tanh_of(__uint_as_float(s[i])));
+  }
+}
 
-namespace masked {
+// s <- f s - slope |far - i| for scores of keys i = 0 .. N - 1 of a query `far` positions behind the first of them.  Where no key that the row
+// sees lies behind it (`linear`) the bias is linear in i: two instructions of the multiply-add pipe for two scores.
+template <int N>
+__device__ __forceinline__ void biased(uint32_t (&s)[N], float f, float slope, float far, bool linear) {
+  if (linear) {
+    const uint64_t f2 = pack_f32x2(f, f), slope2 = pack_f32x2(slope, slope), base2 = pack_f32x2(-slope * far, -slope * far);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t bias = fma_f32x2(slope2, pack_f32x2(static_cast<float>(i), static_cast<float>(i + 1)), base2);
+      float y0, y1;
+      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, bias), y0, y1);
+      s[i] = __float_as_uint(y0), s[i + 1] = __float_as_uint(y1);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), f, -slope * fabsf(far - static_cast<float>(i))));
+  }
+}
 
 // The launch of an instance of the forward kernel; grid: CTAs.  tiles: query tiles of an item, 1 or 2.
 template <int D, bool BF16, bool PAGED>
