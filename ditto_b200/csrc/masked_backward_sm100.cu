@@ -31,10 +31,11 @@ namespace ditto_b200 {
 namespace masked {
 namespace {
 
-constexpr int kComputeWarps = 8, kThreads = 32 * (kComputeWarps + 3);
+constexpr int kComputeWarps = 16, kThreads = 32 * (kComputeWarps + 3);
 constexpr int kProducerWarp = kComputeWarps, kMmaWarp = kComputeWarps + 1;      // (two MMA warps)
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColDp = 128, kColAcc = 256;
 constexpr int kSegs = 4;
+constexpr int kCols = 32;                              // columns of a score tile that one of a row's four threads has
 constexpr float kPScaleLog2 = 14.0f;                   // of P in fp16
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -157,7 +158,7 @@ struct Layout {
 struct Bars {
   uint64_t keep_full, keep_empty;
   uint64_t full[2], empty[2];
-  uint64_t s_full, s_taken, p_full, dp_full[2], ds_full[2], dp_free[2], acc_done, acc_free;
+  uint64_t s_full[2], s_taken, p_full[2], dp_full[2], ds_full[2], dp_free[2], acc_done, acc_free;
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   uint32_t tmem_base, abort_word;
   int start_item, start_tile, left, per_cta;
@@ -245,10 +246,12 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
       mbar_init(&bar->full[i], 1);
       mbar_init(&bar->empty[i], 2);
     }
-    mbar_init(&bar->s_full, 1);
-    mbar_init(&bar->p_full, kComputeWarps);
-    mbar_init(&bar->dp_full[0], 1);
-    mbar_init(&bar->ds_full[0], kComputeWarps);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&bar->s_full[g], 1);
+      mbar_init(&bar->p_full[g], kComputeWarps / 2);
+      mbar_init(&bar->dp_full[g], 1);
+      mbar_init(&bar->ds_full[g], kComputeWarps / 2);
+    }
     mbar_init(&bar->acc_done, 2);
     mbar_init(&bar->acc_free, kComputeWarps);
     for (int i = 0; i < kSegs; ++i) {
@@ -336,28 +339,29 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
     // ------------------------------------------------------------ MMA: warp 0 S^T = K Q^T and dV += P^T dO, warp 1 dP^T = V dO^T and dK += dS^T Q
     const int which = warp - kMmaWarp;
     const uint32_t issuer = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(BF16, kKeys, kRows, false, false);
+    const uint32_t idesc_s = umma_idesc_f16(BF16, kKeys, kRows / 2, false, false);
     const uint32_t idesc_acc = umma_idesc_f16(BF16, kKeys, D, false, true);
     const uint64_t da = umma_desc_sw128(smem_u32(smem + (which == 0 ? LO::kOffA : LO::kOffB)), 16, 1024);
     // the first product's second operand (Q or dO) K-major, the second product's (dO or Q) with the rows as the reduction
     const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kTile), 16, 1024);
     const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + (which ^ 1) * kTile), kRows * 128, 1024);
     const uint32_t d_first = tmem_base + (which == 0 ? kColS : kColDp), d_acc = tmem_base + kColAcc + which * D;
-    uint64_t* first_full = which == 0 ? &bar->s_full : &bar->dp_full[0];
-    uint64_t* back_full = which == 0 ? &bar->p_full : &bar->ds_full[0];
+    uint64_t* first_full = which == 0 ? bar->s_full : bar->dp_full;
+    uint64_t* back_full = which == 0 ? bar->p_full : bar->ds_full;
     auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
       const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
       tc_fence_after_sync();
       return r;
     };
-    auto issue_first = [&](int n) {
-      const uint64_t db = db0 + (((n & 1) * 2 * kTile) >> 4);
+    // the first product of half g of the rows of tile n
+    auto issue_first = [&](int n, int g) {
+      const uint64_t db = db0 + (((n & 1) * 2 * kTile + g * (kRows / 2) * 128) >> 4);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
-        umma_ss_elected(d_first, da + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
+        umma_ss_elected(d_first + g * (kRows / 2), da + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
       }
-      umma_commit_elected(first_full, issuer);
+      umma_commit_elected(&first_full[g], issuer);
     };
     uint32_t keeps = 0;
     int n = 0;
@@ -370,29 +374,37 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
       mbar_arrive_warp(&bar->seg_empty[slot], lane);
       if (lo >= hi) continue;
       if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300) && wait(&bar->full[n & 1], (n >> 1) & 1, 0x310))) break;
-      issue_first(n);
+      issue_first(n, 0);
+      issue_first(n, 1);
       for (int i = lo; i < hi; ++i, ++n) {
-        if (!(ok = wait(back_full, n & 1, 0x340 + which))) break;
-        if (i == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
         const uint64_t dr = dr0 + (((n & 1) * 2 * kTile) >> 4);
 #pragma unroll
-        for (int k = 0; k < kRows / 16; ++k)
-          umma_ts_elected(d_acc, d_first + (k / 4) * 64 + (k % 4) * 8, dr + ((k * 2048) >> 4), idesc_acc, k > 0 || i > lo ? 1u : 0u, issuer);
-        umma_commit_elected(&bar->empty[n & 1], issuer);
-        if (i + 1 < hi) {
-          if (!(ok = wait(&bar->full[(n + 1) & 1], ((n + 1) >> 1) & 1, 0x311))) break;
-          issue_first(n + 1);
+        for (int g = 0; g < 2; ++g) {
+          if (!(ok = ok && wait(&back_full[g], n & 1, 0x340 + which))) break;
+          if (g == 0 && i == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
+#pragma unroll
+          for (int q = 0; q < kRows / 32; ++q)
+            umma_ts_elected(d_acc, d_first + g * (kRows / 2) + (q / 2) * kCols + (q % 2) * 8, dr + (((g * (kRows / 32) + q) * 2048) >> 4), idesc_acc,
+                            g > 0 || q > 0 || i > lo ? 1u : 0u, issuer);
+          if (g == 1) umma_commit_elected(&bar->empty[n & 1], issuer);
+          if (i + 1 < hi) {
+            if (g == 0 && !(ok = wait(&bar->full[(n + 1) & 1], ((n + 1) >> 1) & 1, 0x311))) break;
+            issue_first(n + 1, g);
+          }
         }
+        if (!ok) break;
       }
+      if (!ok) break;
       umma_commit_elected(&bar->keep_empty, issuer);
       umma_commit_elected(&bar->acc_done, issuer);
       ++keeps;
     }
   } else {
-    // ------------------------------------------------------------ arithmetic: thread a key, half of the tile's rows
-    const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+    // ------------------------------------------------------------ arithmetic: thread a key and a quarter of the tile's rows; warps 0-7 the
+    // first half of them, 8-15 the second, each half with buffers of its own
+    const int quad = warp & 3, part_of_row = warp >> 2, g = warp >> 3, row = quad * 32 + lane;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t s_col = lane_base + kColS + half * 64, dp_col = lane_base + kColDp + half * 64;
+    const uint32_t s_col = lane_base + kColS + part_of_row * kCols, dp_col = lane_base + kColDp + part_of_row * kCols;
     const float c = p.c;
     float up, down;
     ds_scale<BF16>(p, &up, &down);
@@ -426,18 +438,17 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         const int st = n & 1;
         const TileRows& rows = *reinterpret_cast<const TileRows*>(smem + LO::kOffRows + st * sizeof(TileRows));
         ok = mbar_wait(&bar->full[st], (n >> 1) & 1, abort_word, 0x850);
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bar->s_full, n & 1, abort_word, 0x800));
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bar->s_full[g], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
-        const int pos0 = p.L - p.M + i * p.tile_tokens;      // of column 0; columns from .. to - 1 of this half see the key
-        const int from = first > pos0 ? min(first - pos0, kRows) * p.group - half * 64 : 0;
-        const int to = min(max(end - pos0, 0), kRows) * p.group - half * 64;
-        const bool cut = __any_sync(0xffffffffu, from > 0), cut_end = __any_sync(0xffffffffu, to < 64);
-        float w[64];
-#pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {
+        const int pos0 = p.L - p.M + i * p.tile_tokens;      // of column 0; columns from .. to - 1 of this thread's see the key
+        const int from = first > pos0 ? min(first - pos0, kRows) * p.group - part_of_row * kCols : 0;
+        const int to = min(max(end - pos0, 0), kRows) * p.group - part_of_row * kCols;
+        const bool cut = __any_sync(0xffffffffu, from > 0), cut_end = __any_sync(0xffffffffu, to < kCols);
+        float w[kCols];
+        {
           uint32_t sv[32];
-          tmem_ld_x32_wait(s_col + ch * 32, sv);
+          tmem_ld_x32_wait(s_col, sv);
           // (w holds what dS is the product of with dP - delta: first 1 - tanh^2, then that times the weight)
           if constexpr (GENERAL) {
             if (p.cap_out != 0.f) {
@@ -446,22 +457,22 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
 #pragma unroll
               for (int u = 0; u < 32; u += 2) {
                 const uint64_t t = pack_f32x2(__uint_as_float(sv[u]), __uint_as_float(sv[u + 1]));
-                unpack_f32x2(fma_f32x2(mul_f32x2(t, pack_f32x2(-1.0f, -1.0f)), t, one2), w[ch * 32 + u], w[ch * 32 + u + 1]);
+                unpack_f32x2(fma_f32x2(mul_f32x2(t, pack_f32x2(-1.0f, -1.0f)), t, one2), w[u], w[u + 1]);
                 float y0, y1;
                 unpack_f32x2(mul_f32x2(t, out2), y0, y1);
                 sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
             } else {
 #pragma unroll
-              for (int u = 0; u < 32; ++u) w[ch * 32 + u] = 1.0f;
+              for (int u = 0; u < 32; ++u) w[u] = 1.0f;
             }
             if (p.slopes != nullptr) {
               const float sc = p.cap_out != 0.f ? 1.0f : p.score_log2, at = static_cast<float>(key);
               const uint64_t sc2 = pack_f32x2(sc, sc), at2 = pack_f32x2(-at, -at);
 #pragma unroll
               for (int u = 0; u < 32; u += 4) {
-                const float4 sl = *reinterpret_cast<const float4*>(&rows.slope[half * 64 + ch * 32 + u]);
-                const float4 ps = *reinterpret_cast<const float4*>(&rows.pos[half * 64 + ch * 32 + u]);
+                const float4 sl = *reinterpret_cast<const float4*>(&rows.slope[part_of_row * kCols + u]);
+                const float4 ps = *reinterpret_cast<const float4*>(&rows.pos[part_of_row * kCols + u]);
 #pragma unroll
                 for (int q = 0; q < 4; q += 2) {
                   float d0, d1;
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
           if (mixed) {
 #pragma unroll
               for (int u = 0; u < 32; u += 4) {
-                const int4 d = *reinterpret_cast<const int4*>(&rows.doc[half * 64 + ch * 32 + u]);
+                const int4 d = *reinterpret_cast<const int4*>(&rows.doc[part_of_row * kCols + u]);
                 if (d.x != doc) sv[u] = __float_as_uint(-INFINITY);
                 if (d.y != doc) sv[u + 1] = __float_as_uint(-INFINITY);
                 if (d.z != doc) sv[u + 2] = __float_as_uint(-INFINITY);
@@ -487,12 +498,12 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
           if (cut) {
 #pragma unroll
             for (int u = 0; u < 32; ++u)
-              if (ch * 32 + u < from) sv[u] = __float_as_uint(-INFINITY);
+              if (u < from) sv[u] = __float_as_uint(-INFINITY);
           }
           if (cut_end) {
 #pragma unroll
             for (int u = 0; u < 32; ++u)
-              if (ch * 32 + u >= to) sv[u] = __float_as_uint(-INFINITY);
+              if (u >= to) sv[u] = __float_as_uint(-INFINITY);
           }
           const uint64_t c2 = pack_f32x2(c, c);
 #pragma unroll
@@ -501,50 +512,49 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
 #pragma unroll
             for (int v = 0; v < 8; v += 2) {
               const int u = q * 16 + v * 2;
-              const float4 lse = *reinterpret_cast<const float4*>(&rows.lse[half * 64 + ch * 32 + u]);
+              const float4 lse = *reinterpret_cast<const float4*>(&rows.lse[part_of_row * kCols + u]);
               float p0, p1, p2, p3;
               unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, pack_f32x2(p_log2 - lse.x, p_log2 - lse.y), false), p0, p1);
               unpack_f32x2(softmax_weights(sv[u + 2], sv[u + 3], c2, pack_f32x2(p_log2 - lse.z, p_log2 - lse.w), weights_on_fma(u / 2 + 1)), p2, p3);
               pk[v] = pack2<BF16>(p0, p1);
               pk[v + 1] = pack2<BF16>(p2, p3);
-              const int x = ch * 32 + u;
+              const int x = u;
               w[x] = GENERAL ? p0 * w[x] : p0, w[x + 1] = GENERAL ? p1 * w[x + 1] : p1;
               w[x + 2] = GENERAL ? p2 * w[x + 2] : p2, w[x + 3] = GENERAL ? p3 * w[x + 3] : p3;
             }
-            // (packed weights go over the first half of this half's own columns)
-            tmem_st_x8(s_col + ch * 16 + q * 8, pk);
+            // (packed weights go over the first half of this thread's own columns)
+            tmem_st_x8(s_col + q * 8, pk);
           }
         }
         tmem_wait_st();
         tc_fence_before_sync();
-        mbar_arrive_warp(&bar->p_full, lane);
+        mbar_arrive_warp(&bar->p_full[g], lane);
 
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[0], n & 1, abort_word, 0x810));
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[g], n & 1, abort_word, 0x810));
         if (!ok) break;
         tc_fence_after_sync();
-#pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {
+        {
           uint32_t dp[32];
-          tmem_ld_x32_wait(dp_col + ch * 32, dp);
+          tmem_ld_x32_wait(dp_col, dp);
           uint32_t pk[16];
 #pragma unroll
           for (int u = 0; u < 32; u += 4) {
-            const float4 de = *reinterpret_cast<const float4*>(&rows.delta[half * 64 + ch * 32 + u]);
-            const int x = ch * 32 + u;
+            const float4 de = *reinterpret_cast<const float4*>(&rows.delta[part_of_row * kCols + u]);
+            const int x = u;
             const float f0 = BF16 ? w[x] : w[x] * f, f1 = BF16 ? w[x + 1] : w[x + 1] * f, f2 = BF16 ? w[x + 2] : w[x + 2] * f,
                         f3 = BF16 ? w[x + 3] : w[x + 3] * f;
             pk[u / 2] = pack2<BF16>(f0 * (__uint_as_float(dp[u]) - de.x), f1 * (__uint_as_float(dp[u + 1]) - de.y));
             pk[u / 2 + 1] = pack2<BF16>(f2 * (__uint_as_float(dp[u + 2]) - de.z), f3 * (__uint_as_float(dp[u + 3]) - de.w));
           }
-          tmem_st_x16(dp_col + ch * 16, pk);
+          tmem_st_x16(dp_col, pk);
         }
         tmem_wait_st();
         tc_fence_before_sync();
-        mbar_arrive_warp(&bar->ds_full[0], lane);
+        mbar_arrive_warp(&bar->ds_full[g], lane);
       }
       if (!ok) break;
 
-      // the block's gradients, or this part of their sums: dV in the first D columns, dK behind them; half of the columns a thread
+      // the block's gradients, or this part of their sums: dV in the first D columns, dK behind them; a quarter of the columns a thread
       const bool has = lo < hi;
       if (has) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->acc_done, accs & 1, abort_word, 0x830));
@@ -558,27 +568,27 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         uint8_t* dst = static_cast<uint8_t*>(m == 0 ? p.dv : p.dk) + 2 * ((static_cast<size_t>(s.seq) * p.L + key) * p.kv_heads + s.kv_head) * p.d;
         float* part = p.part + (((static_cast<size_t>(blockIdx.x) * 2 + max(s.part, 0)) * 2 + m) * kKeys + row) * D;
 #pragma unroll
-        for (int cc = 0; cc < D / 2; cc += 32) {
-          const int col = half * (D / 2) + cc;
-          uint32_t x[32];
+        for (int cc = 0; cc < D / 4; cc += 16) {
+          const int col = part_of_row * (D / 4) + cc;
+          uint32_t x[16];
           if (has) {
-            tmem_ld_x32_wait(lane_base + kColAcc + m * D + col, x);
+            tmem_ld_x16_wait(lane_base + kColAcc + m * D + col, x);
           } else {
 #pragma unroll
-            for (int u = 0; u < 32; ++u) x[u] = 0u;
+            for (int u = 0; u < 16; ++u) x[u] = 0u;
           }
-          if (m == 1 && cc + 32 == D / 2) {
+          if (m == 1 && cc + 16 == D / 4) {
             tc_fence_before_sync();
             if (has) mbar_arrive_warp(&bar->acc_free, lane);
           }
           if (key >= p.L) continue;
           if (s.part >= 0) {
 #pragma unroll
-            for (int u = 0; u < 32; u += 4) *reinterpret_cast<uint4*>(part + col + u) = make_uint4(x[u], x[u + 1], x[u + 2], x[u + 3]);
+            for (int u = 0; u < 16; u += 4) *reinterpret_cast<uint4*>(part + col + u) = make_uint4(x[u], x[u + 1], x[u + 2], x[u + 3]);
             continue;
           }
 #pragma unroll
-          for (int u = 0; u < 32; u += 8) {
+          for (int u = 0; u < 16; u += 8) {
             uint32_t v[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) v[q] = pack2<BF16>(__uint_as_float(x[u + 2 * q]) * scale, __uint_as_float(x[u + 2 * q + 1]) * scale);
@@ -661,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       mbar_init(&bar->ds_full[i], kComputeWarps);
       mbar_init(&bar->dp_free[i], 1);
     }
-    mbar_init(&bar->s_full, 1);
+    mbar_init(&bar->s_full[0], 1);
     mbar_init(&bar->s_taken, kComputeWarps);
     mbar_init(&bar->acc_done, 1);
     mbar_init(&bar->acc_free, kComputeWarps);
@@ -764,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
           const uint64_t dk = dk0 + ((st * 2 * kTile) >> 4);
           if (!(ok = wait(&bar->full[st], two, 0x310) && wait(&bar->s_taken, (n & 1) ^ 1, 0x330))) break;
           scores(tmem_base + kColS, dq, dk);
-          umma_commit_elected(&bar->s_full, issuer);
+          umma_commit_elected(&bar->s_full[0], issuer);
           if (!(ok = wait(&bar->dp_free[st], two ^ 1, 0x331))) break;
           scores(tmem_base + (st ? kColDp1 : kColDp), ddo, dk + (kTile >> 4));
           umma_commit_elected(&bar->dp_full[st], issuer);
@@ -780,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
           const uint32_t a = tmem_base + (st ? kColDp1 : kColDp);
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
-            umma_ts_elected(tmem_base + kColAcc, a + (k / 4) * 64 + (k % 4) * 8, dr + ((k * 2048) >> 4), idesc_acc, k > 0 || j > lo ? 1u : 0u, issuer);
+            umma_ts_elected(tmem_base + kColAcc, a + (k / 2) * kCols + (k % 2) * 8, dr + ((k * 2048) >> 4), idesc_acc, k > 0 || j > lo ? 1u : 0u, issuer);
           umma_commit_elected(&bar->dp_free[st], issuer);
           umma_commit_elected(&bar->empty[st], issuer);
         }
@@ -789,8 +799,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       ++keeps;
     }
   } else {
-    // ------------------------------------------------------------ arithmetic: thread a row, half of the block's keys
-    const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;
+    // ------------------------------------------------------------ arithmetic: thread a row and a quarter of the block's keys
+    const int quad = warp & 3, part_of_row = warp >> 2, row = quad * 32 + lane;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = p.c;
     float up, down;
@@ -825,16 +835,15 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       const bool behind = p.causal && s.prefix <= s.keys - s.tokens + s.first_token + 1;      // every key that a row sees is at or in front of it
       for (int j = lo; j < hi; ++j, ++n) {
         const int st = n & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full, n & 1, abort_word, 0x800));
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[0], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
-        const int k0 = j * kKeys + half * 64;
-        const bool cut = __any_sync(0xffffffffu, limit < k0 + 64), cut_low = __any_sync(0xffffffffu, low > k0);
-        float w[64];
-#pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {
+        const int k0 = j * kKeys + part_of_row * kCols;
+        const bool cut = __any_sync(0xffffffffu, limit < k0 + kCols), cut_low = __any_sync(0xffffffffu, low > k0);
+        float w[kCols];
+        {
           uint32_t sv[32];
-          tmem_ld_x32_wait(lane_base + kColS + half * 64 + ch * 32, sv);
+          tmem_ld_x32_wait(lane_base + kColS + part_of_row * kCols, sv);
           if constexpr (GENERAL) {
             if (p.cap_out != 0.f) {
               capped(sv, p.cap_in, 1.0f);
@@ -842,32 +851,32 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
 #pragma unroll
               for (int u = 0; u < 32; u += 2) {
                 const uint64_t t = pack_f32x2(__uint_as_float(sv[u]), __uint_as_float(sv[u + 1]));
-                unpack_f32x2(fma_f32x2(mul_f32x2(t, pack_f32x2(-1.0f, -1.0f)), t, one2), w[ch * 32 + u], w[ch * 32 + u + 1]);
+                unpack_f32x2(fma_f32x2(mul_f32x2(t, pack_f32x2(-1.0f, -1.0f)), t, one2), w[u], w[u + 1]);
                 float y0, y1;
                 unpack_f32x2(mul_f32x2(t, out2), y0, y1);
                 sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
             } else {
 #pragma unroll
-              for (int u = 0; u < 32; ++u) w[ch * 32 + u] = 1.0f;
+              for (int u = 0; u < 32; ++u) w[u] = 1.0f;
             }
-            if (p.slopes != nullptr) biased(sv, p.cap_out != 0.f ? 1.0f : p.score_log2, -slope, static_cast<float>(pos - k0 - ch * 32), behind);
+            if (p.slopes != nullptr) biased(sv, p.cap_out != 0.f ? 1.0f : p.score_log2, -slope, static_cast<float>(pos - k0), behind);
           }
           if (mixed) {
             const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
 #pragma unroll
             for (int u = 0; u < 32; ++u) {
-              if (ids[min(k0 + ch * 32 + u, p.L - 1)] != doc) sv[u] = __float_as_uint(-INFINITY);
+              if (ids[min(k0 + u, p.L - 1)] != doc) sv[u] = __float_as_uint(-INFINITY);
               if (u % 8 == 7) asm volatile("" ::: "memory");       // (eight ids at a time: registers)
             }
           }
           if (cut_low) {
 #pragma unroll
             for (int u = 0; u < 32; ++u)
-              if (u < low - k0 - ch * 32) sv[u] = __float_as_uint(-INFINITY);
+              if (u < low - k0) sv[u] = __float_as_uint(-INFINITY);
           }
           if (cut) {
-            const int lim = limit - k0 - ch * 32;
+            const int lim = limit - k0;
 #pragma unroll
             for (int u = 0; u < 32; ++u)
               if (u >= lim) sv[u] = __float_as_uint(-INFINITY);
@@ -877,8 +886,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
           for (int u = 0; u < 32; u += 2) {
             float p0, p1;
             unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, off2, weights_on_fma(u / 2)), p0, p1);
-            w[ch * 32 + u] = GENERAL ? p0 * w[ch * 32 + u] : p0;
-            w[ch * 32 + u + 1] = GENERAL ? p1 * w[ch * 32 + u + 1] : p1;
+            w[u] = GENERAL ? p0 * w[u] : p0;
+            w[u + 1] = GENERAL ? p1 * w[u + 1] : p1;
           }
         }
         tc_fence_before_sync();
@@ -887,17 +896,16 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[st], (n >> 1) & 1, abort_word, 0x810));
         if (!ok) break;
         tc_fence_after_sync();
-        const uint32_t dp_col = lane_base + (st ? kColDp1 : kColDp) + half * 64;
-#pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {
+        const uint32_t dp_col = lane_base + (st ? kColDp1 : kColDp) + part_of_row * kCols;
+        {
           uint32_t dp[32], pk[16];
-          tmem_ld_x32_wait(dp_col + ch * 32, dp);
+          tmem_ld_x32_wait(dp_col, dp);
 #pragma unroll
           for (int u = 0; u < 32; u += 2) {
-            const float w0 = BF16 ? w[ch * 32 + u] : w[ch * 32 + u] * f, w1 = BF16 ? w[ch * 32 + u + 1] : w[ch * 32 + u + 1] * f;
+            const float w0 = BF16 ? w[u] : w[u] * f, w1 = BF16 ? w[u + 1] : w[u + 1] * f;
             pk[u / 2] = pack2<BF16>(w0 * (__uint_as_float(dp[u]) - delta), w1 * (__uint_as_float(dp[u + 1]) - delta));
           }
-          tmem_st_x16(dp_col + ch * 16, pk);
+          tmem_st_x16(dp_col, pk);
         }
         tmem_wait_st();
         tc_fence_before_sync();
@@ -915,22 +923,22 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       const float scale = p.scale * down;
       uint8_t* dst = static_cast<uint8_t*>(p.dq) + 2 * ((static_cast<size_t>(s.seq) * p.M + token) * p.heads + s.kv_head * p.group + r_head) * p.d;
 #pragma unroll
-      for (int cc = 0; cc < D / 2; cc += 32) {
-        const int col = half * (D / 2) + cc;
-        uint32_t x[32];
+      for (int cc = 0; cc < D / 4; cc += 16) {
+        const int col = part_of_row * (D / 4) + cc;
+        uint32_t x[16];
         if (has) {
-          tmem_ld_x32_wait(lane_base + kColAcc + col, x);
+          tmem_ld_x16_wait(lane_base + kColAcc + col, x);
         } else {
 #pragma unroll
-          for (int u = 0; u < 32; ++u) x[u] = 0u;
+          for (int u = 0; u < 16; ++u) x[u] = 0u;
         }
-        if (cc + 32 == D / 2) {
+        if (cc + 16 == D / 4) {
           tc_fence_before_sync();
           if (has) mbar_arrive_warp(&bar->acc_free, lane);
         }
         if (!valid) continue;
 #pragma unroll
-        for (int u = 0; u < 32; u += 8) {
+        for (int u = 0; u < 16; u += 8) {
           uint32_t v[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) v[q] = pack2<BF16>(__uint_as_float(x[u + 2 * q]) * scale, __uint_as_float(x[u + 2 * q + 1]) * scale);
