@@ -84,9 +84,13 @@ struct MaskedScratch {
   size_t rows, norms, part, parts;       // of the backward pass
   size_t bytes;
 };
+// Tokens of a query tile of the gradient kernels.
+int backward_tokens(int group) { return group <= masked::kHalf ? 2 * (masked::kHalf / group) : 1; }
+
 MaskedScratch masked_scratch(const ditto_b200_masked_args* a, bool backward, int sms) {
   MaskedScratch s = {};
-  const size_t blocks = (a->L + 127) / 128, tile_tokens = 128 / (a->heads / a->kv_heads), tiles = (a->M + tile_tokens - 1) / tile_tokens;
+  const int group = a->heads / a->kv_heads;
+  const size_t blocks = (a->L + 127) / 128, tile_tokens = backward ? backward_tokens(group) : 128 / group, tiles = (a->M + tile_tokens - 1) / tile_tokens;
   if (a->documents != nullptr) {
     s.mixed = up256(static_cast<size_t>(a->batch) * a->L * sizeof(int2));
     s.key_blocks = s.mixed + up256(a->batch * sizeof(int));
@@ -96,7 +100,7 @@ MaskedScratch masked_scratch(const ditto_b200_masked_args* a, bool backward, int
   }
   if (backward) {
     s.rows = s.bytes;
-    s.norms = s.rows + up256(a->batch * a->kv_heads * tiles * sizeof(masked::TileRows));
+    s.norms = s.rows + up256(a->batch * a->kv_heads * tiles * 2 * sizeof(masked::HalfRows));
     s.part = s.norms + 256;
     s.parts = s.part + static_cast<size_t>(sms) * 2 * 2 * 128 * (a->head_dim <= 64 ? 64 : 128) * sizeof(float);
     s.bytes = s.parts + up256(sms * sizeof(masked::KeyPartDesc));
@@ -274,10 +278,21 @@ int ditto_b200_masked_attention_backward(const ditto_b200_masked_args* a, const 
   const bool bf16 = a->dtype == DITTO_DTYPE_BF16;
   masked::BackwardParams p;
   std::memset(&p, 0, sizeof(p));
-  p.map_q = f.map_q;
-  p.map_k = f.map_k;
-  p.map_v = f.map_v;
-  rc = map_4d(&p.map_do, bf16, grad_out, f.d, f.heads, f.M, f.batch, grad_strides[2], grad_strides[1], grad_strides[0], f.group, f.tile_tokens);
+  // halves of a tile: whole tokens, or half of one token's heads
+  p.half_heads = f.group <= masked::kHalf ? f.group : (f.group + 1) / 2;
+  p.head_step = f.group <= masked::kHalf ? 0 : p.half_heads;
+  const int box_tokens = f.group <= masked::kHalf ? masked::kHalf / f.group : 1;
+  p.half_tokens = f.group <= masked::kHalf ? box_tokens : 0;
+  p.half_rows = p.half_heads * box_tokens;
+  f.tile_tokens = backward_tokens(f.group);
+  f.tiles = (f.M + f.tile_tokens - 1) / f.tile_tokens;
+  rc = map_4d(&p.map_q, bf16, a->q, f.d, f.heads, f.M, f.batch, a->q_strides[2], a->q_strides[1], a->q_strides[0], p.half_heads, box_tokens);
+  if (rc) return rc;
+  rc = map_4d(&p.map_do, bf16, grad_out, f.d, f.heads, f.M, f.batch, grad_strides[2], grad_strides[1], grad_strides[0], p.half_heads, box_tokens);
+  if (rc) return rc;
+  rc = map_4d(&p.map_k, bf16, a->k, f.d, f.L, f.kv_heads, f.batch, a->k_strides[1], a->k_strides[2], a->k_strides[0], 64, 1);
+  if (rc) return rc;
+  rc = map_4d(&p.map_v, bf16, a->v, f.d, f.L, f.kv_heads, f.batch, a->v_strides[1], a->v_strides[2], a->v_strides[0], 64, 1);
   if (rc) return rc;
   p.o = a->out;
   p.grad = grad_out;
@@ -301,7 +316,7 @@ int ditto_b200_masked_attention_backward(const ditto_b200_masked_args* a, const 
   p.slopes = f.slopes, p.prefix = f.prefix, p.documents = f.documents;
   p.status = status_word;
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  p.rows = reinterpret_cast<masked::TileRows*>(base + ws.rows);
+  p.rows = reinterpret_cast<masked::HalfRows*>(base + ws.rows);
   p.norms = reinterpret_cast<uint32_t*>(base + ws.norms);
   p.part = reinterpret_cast<float*>(base + ws.part);
   p.parts = reinterpret_cast<masked::KeyPartDesc*>(base + ws.parts);

@@ -83,13 +83,14 @@ __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid
   float norm_g = 0.f, norm_v = 0.f;
   // (the loops' bounds are those of whole warps: shuffles)
   for (long long at = static_cast<long long>(blockIdx.x) * (kRowThreads / 16) + threadIdx.x / 16; at - (threadIdx.x / 16 & 1) < rows; at += step) {
-    const int r = static_cast<int>(at % kRows);
+    const int r = static_cast<int>(at % kHalf), g = static_cast<int>(at / kHalf % 2);
     long long rest = at / kRows;
     const int tile = static_cast<int>(rest % p.tiles);
     rest /= p.tiles;
     const int kv_head = static_cast<int>(rest % p.kv_heads), b = static_cast<int>(rest / p.kv_heads);
-    const int token = tile * p.tile_tokens + r / p.group, head = kv_head * p.group + r % p.group, pos = token + p.L - p.M;
-    const bool valid = at < rows && r / p.group < p.tile_tokens && token < p.M;
+    const int token = tile * p.tile_tokens + g * p.half_tokens + r / p.half_heads, in_group = g * p.head_step + r % p.half_heads;
+    const int head = kv_head * p.group + in_group, pos = token + p.L - p.M;
+    const bool valid = at < rows && r < p.half_rows && in_group < p.group && token < p.M;
     float dot = 0.f, norm = 0.f;
     if (valid && lane < pieces) {
       const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.grad) + 2 * (b * p.g_stride[0] + token * p.g_stride[1] + head * p.g_stride[2]) + lane * 16);
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid
     }
     norm_g = fmaxf(norm_g, norm);
     if (lane == 0 && at < rows) {
-      TileRows& t = p.rows[at / kRows];
+      HalfRows& t = p.rows[at / kHalf];
       const float lse = valid ? p.lse[(static_cast<size_t>(b) * p.M + token) * p.heads + head] : -INFINITY;
       t.lse[r] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
       t.delta[r] = dot;
@@ -148,17 +149,18 @@ template <int D>
 struct Layout {
   static constexpr int kAtoms = D / 64, kTile = 128 * D * 2;
   static constexpr int kOffA = 0, kOffB = kTile;                 // what stays: K and V, or Q and dO
-  static constexpr int kOffRing = 2 * kTile;                     // two stages of what passes: Q and dO, or K and V
-  static constexpr int kOffRows = kOffRing + 4 * kTile;          // [2] TileRows
-  static constexpr int kOffBar = kOffRows + 2 * static_cast<int>(sizeof(TileRows));
+  static constexpr int kHalfTile = kTile / 2;
+  static constexpr int kOffRing = 2 * kTile;                     // four stages of what passes: halves of Q and dO, or of K and V
+  static constexpr int kOffRows = kOffRing + 4 * kTile;          // [4] HalfRows
+  static constexpr int kOffBar = kOffRows + 4 * static_cast<int>(sizeof(HalfRows));
   static constexpr int kOffSeg = kOffBar + 512;
   static constexpr int kBytes = kOffSeg + 512 + 1024;
 };
 
 struct Bars {
   uint64_t keep_full, keep_empty;
-  uint64_t full[2], empty[2];
-  uint64_t s_full[2], s_taken, p_full[2], dp_full[2], ds_full[2], dp_free[2], acc_done, acc_free;
+  uint64_t full[4], empty[4];
+  uint64_t s_full[2], s_taken[2], p_full[2], dp_full[2], ds_full[2], acc_done, acc_free;
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   uint32_t tmem_base, abort_word;
   int start_item, start_tile, left, per_cta;
@@ -218,11 +220,18 @@ __device__ __forceinline__ void find_share(const BackwardParams& p, Bars* bar) {
   __syncthreads();
 }
 
-__device__ __forceinline__ void zero_unused_rows(uint8_t* tile, int atoms, int from) {
-  // rows of a query tile that the loads do not write (a group that does not divide 128): as rows of the sums they have to be zeros
+// Rows of a half that the loads do not write (a group that does not divide 64): as rows of the sums they have to be zeros.
+__device__ __forceinline__ void zero_unused_rows(uint8_t* half, int atoms, int from) {
   for (int a = 0; a < atoms; ++a)
-    for (int i = from * 8 + static_cast<int>(threadIdx.x); i < kRows * 8; i += kThreads)
-      *reinterpret_cast<uint4*>(tile + a * (kRows * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+    for (int i = from * 8 + static_cast<int>(threadIdx.x); i < kHalf * 8; i += kThreads)
+      *reinterpret_cast<uint4*>(half + a * (kHalf * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// 128 rows of keys, or of queries (`heads` apart from the one that tokens step by), in two boxes of 64.
+template <int D>
+__device__ __forceinline__ void load_halves(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int x1, int x1_step, int x2, int x2_step, int x3) {
+  for (int a = 0; a < D / 64; ++a)
+    for (int g = 0; g < 2; ++g) tma_load_4d(dst + a * (kRows * 128) + g * (kHalf * 128), map, bar, a * 64, x1 + g * x1_step, x2 + g * x2_step, x3);
 }
 
 }  // namespace
@@ -231,7 +240,7 @@ __device__ __forceinline__ void zero_unused_rows(uint8_t* tile, int atoms, int f
 template <int D, bool BF16, bool GENERAL>
 __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid_constant__ BackwardParams p) {
   using LO = Layout<D>;
-  constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile;
+  constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile, kHalfTile = LO::kHalfTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars* bar = reinterpret_cast<Bars*>(smem + LO::kOffBar);
@@ -242,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
   if (threadIdx.x == 0) {
     mbar_init(&bar->keep_full, 1);
     mbar_init(&bar->keep_empty, 2);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bar->full[i], 1);
       mbar_init(&bar->empty[i], 2);
     }
@@ -265,8 +274,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
     tmem_alloc(&bar->tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  if (p.group * p.tile_tokens < kRows) {
-    for (int i = 0; i < 4; ++i) zero_unused_rows(smem + LO::kOffRing + i * kTile, kAtoms, p.group * p.tile_tokens);
+  if (p.half_rows < kHalf) {
+    for (int i = 0; i < 8; ++i) zero_unused_rows(smem + LO::kOffRing + i * kHalfTile, kAtoms, p.half_rows);
     fence_proxy_async_smem();
   }
   tc_fence_before_sync();
@@ -280,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      const uint32_t tile_bytes = static_cast<uint32_t>(p.group * p.tile_tokens) * 128 * kAtoms;
+      const uint32_t half_bytes = static_cast<uint32_t>(p.half_rows) * 128 * kAtoms;
       int item = bar->start_item, skip = bar->start_tile, left = bar->left, done = 0, n = 0, keeps = 0;
       bool ok = true;
       for (int segs = 0; ok; ++segs) {
@@ -316,22 +325,23 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         if (!ok) break;
         ++keeps;
         mbar_arrive_expect_tx(&bar->keep_full, 2 * kTile);
-        for (int a = 0; a < kAtoms; ++a) {
-          tma_load_4d(smem + LO::kOffA + a * (kKeys * 128), &p.map_k, &bar->keep_full, a * 64, s.block * kKeys, s.kv_head, s.seq);
-          tma_load_4d(smem + LO::kOffB + a * (kKeys * 128), &p.map_v, &bar->keep_full, a * 64, s.block * kKeys, s.kv_head, s.seq);
-        }
-        for (int i = s.lo; i < s.hi; ++i, ++n) {
-          const int st = n & 1;
-          ok = mbar_wait(&bar->empty[st], ((n >> 1) & 1) ^ 1, abort_word, 0x110);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&bar->full[st], 2 * tile_bytes + static_cast<uint32_t>(sizeof(TileRows)));
-          uint8_t* dst = smem + LO::kOffRing + st * 2 * kTile;
-          for (int a = 0; a < kAtoms; ++a) {
-            tma_load_4d(dst + a * (kRows * 128), &p.map_q, &bar->full[st], a * 64, s.kv_head * p.group, i * p.tile_tokens, s.seq);
-            tma_load_4d(dst + kTile + a * (kRows * 128), &p.map_do, &bar->full[st], a * 64, s.kv_head * p.group, i * p.tile_tokens, s.seq);
+        load_halves<D>(smem + LO::kOffA, &p.map_k, &bar->keep_full, s.block * kKeys, kHalf, s.kv_head, 0, s.seq);
+        load_halves<D>(smem + LO::kOffB, &p.map_v, &bar->keep_full, s.block * kKeys, kHalf, s.kv_head, 0, s.seq);
+        for (int i = s.lo; ok && i < s.hi; ++i, ++n) {
+          for (int g = 0; g < 2; ++g) {
+            const int h = 2 * n + g, st = h & 3;
+            ok = mbar_wait(&bar->empty[st], ((h >> 2) & 1) ^ 1, abort_word, 0x110);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&bar->full[st], 2 * half_bytes + static_cast<uint32_t>(sizeof(HalfRows)));
+            uint8_t* dst = smem + LO::kOffRing + st * kTile;
+            const int head = s.kv_head * p.group + g * p.head_step, token = i * p.tile_tokens + g * p.half_tokens;
+            for (int a = 0; a < kAtoms; ++a) {
+              tma_load_4d(dst + a * (kHalf * 128), &p.map_q, &bar->full[st], a * 64, head, token, s.seq);
+              tma_load_4d(dst + kHalfTile + a * (kHalf * 128), &p.map_do, &bar->full[st], a * 64, head, token, s.seq);
+            }
+            bulk_load(smem + LO::kOffRows + st * sizeof(HalfRows), p.rows + ((static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + i) * 2 + g,
+                      sizeof(HalfRows), &bar->full[st]);
           }
-          bulk_load(smem + LO::kOffRows + st * sizeof(TileRows), p.rows + (static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + i,
-                    sizeof(TileRows), &bar->full[st]);
         }
       }
     }
@@ -339,12 +349,12 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
     // ------------------------------------------------------------ MMA: warp 0 S^T = K Q^T and dV += P^T dO, warp 1 dP^T = V dO^T and dK += dS^T Q
     const int which = warp - kMmaWarp;
     const uint32_t issuer = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(BF16, kKeys, kRows / 2, false, false);
+    const uint32_t idesc_s = umma_idesc_f16(BF16, kKeys, kHalf, false, false);
     const uint32_t idesc_acc = umma_idesc_f16(BF16, kKeys, D, false, true);
     const uint64_t da = umma_desc_sw128(smem_u32(smem + (which == 0 ? LO::kOffA : LO::kOffB)), 16, 1024);
     // the first product's second operand (Q or dO) K-major, the second product's (dO or Q) with the rows as the reduction
-    const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kTile), 16, 1024);
-    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + (which ^ 1) * kTile), kRows * 128, 1024);
+    const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kHalfTile), 16, 1024);
+    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + (which ^ 1) * kHalfTile), kHalf * 128, 1024);
     const uint32_t d_first = tmem_base + (which == 0 ? kColS : kColDp), d_acc = tmem_base + kColAcc + which * D;
     uint64_t* first_full = which == 0 ? bar->s_full : bar->dp_full;
     uint64_t* back_full = which == 0 ? bar->p_full : bar->ds_full;
@@ -353,16 +363,16 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
       tc_fence_after_sync();
       return r;
     };
-    // the first product of half g of the rows of tile n
+    // the first product of half g of the rows of tile n: stage 2 n + g of the ring
     auto issue_first = [&](int n, int g) {
-      const uint64_t db = db0 + (((n & 1) * 2 * kTile + g * (kRows / 2) * 128) >> 4);
+      const uint64_t db = db0 + ((((2 * n + g) & 3) * kTile) >> 4);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
-        umma_ss_elected(d_first + g * (kRows / 2), da + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
-      }
+      for (int i = 0; i < D / 16; ++i)
+        umma_ss_elected(d_first + g * kHalf, da + (((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4), db + (((i / 4) * (kHalf * 128) + (i % 4) * 32) >> 4),
+                        idesc_s, i > 0 ? 1u : 0u, issuer);
       umma_commit_elected(&first_full[g], issuer);
     };
+    auto wait_half = [&](int n, int g) { return wait(&bar->full[(2 * n + g) & 3], (n >> 1) & 1, 0x310 + g); };
     uint32_t keeps = 0;
     int n = 0;
     bool ok = true;
@@ -373,22 +383,23 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
       const int lo = segments[slot].lo, hi = segments[slot].hi;
       mbar_arrive_warp(&bar->seg_empty[slot], lane);
       if (lo >= hi) continue;
-      if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300) && wait(&bar->full[n & 1], (n >> 1) & 1, 0x310))) break;
+      if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300) && wait_half(n, 0))) break;
       issue_first(n, 0);
+      if (!(ok = wait_half(n, 1))) break;
       issue_first(n, 1);
       for (int i = lo; i < hi; ++i, ++n) {
-        const uint64_t dr = dr0 + (((n & 1) * 2 * kTile) >> 4);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
+          const uint64_t dr = dr0 + ((((2 * n + g) & 3) * kTile) >> 4);
           if (!(ok = ok && wait(&back_full[g], n & 1, 0x340 + which))) break;
           if (g == 0 && i == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
 #pragma unroll
-          for (int q = 0; q < kRows / 32; ++q)
-            umma_ts_elected(d_acc, d_first + g * (kRows / 2) + (q / 2) * kCols + (q % 2) * 8, dr + (((g * (kRows / 32) + q) * 2048) >> 4), idesc_acc,
+          for (int q = 0; q < kHalf / 16; ++q)
+            umma_ts_elected(d_acc, d_first + g * kHalf + (q / 2) * kCols + (q % 2) * 8, dr + ((q * 2048) >> 4), idesc_acc,
                             g > 0 || q > 0 || i > lo ? 1u : 0u, issuer);
-          if (g == 1) umma_commit_elected(&bar->empty[n & 1], issuer);
+          umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
           if (i + 1 < hi) {
-            if (g == 0 && !(ok = wait(&bar->full[(n + 1) & 1], ((n + 1) >> 1) & 1, 0x311))) break;
+            if (!(ok = wait_half(n + 1, g))) break;
             issue_first(n + 1, g);
           }
         }
@@ -402,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
   } else {
     // ------------------------------------------------------------ arithmetic: thread a key and a quarter of the tile's rows; warps 0-7 the
     // first half of them, 8-15 the second, each half with buffers of its own
-    const int quad = warp & 3, part_of_row = warp >> 2, g = warp >> 3, row = quad * 32 + lane;
+    const int quad = warp & 3, part_of_row = warp >> 2, g = warp >> 3, sub = part_of_row & 1, row = quad * 32 + lane;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t s_col = lane_base + kColS + part_of_row * kCols, dp_col = lane_base + kColDp + part_of_row * kCols;
     const float c = p.c;
@@ -435,15 +446,15 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         mixed = p.mixed[s.seq] != 0;
       }
       for (int i = lo; i < hi; ++i, ++n) {
-        const int st = n & 1;
-        const TileRows& rows = *reinterpret_cast<const TileRows*>(smem + LO::kOffRows + st * sizeof(TileRows));
+        const int st = (2 * n + g) & 3;
+        const HalfRows& rows = *reinterpret_cast<const HalfRows*>(smem + LO::kOffRows + st * sizeof(HalfRows));
         ok = mbar_wait(&bar->full[st], (n >> 1) & 1, abort_word, 0x850);
         ok = __all_sync(0xffffffffu, ok && mbar_wait(&bar->s_full[g], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
-        const int pos0 = p.L - p.M + i * p.tile_tokens;      // of column 0; columns from .. to - 1 of this thread's see the key
-        const int from = first > pos0 ? min(first - pos0, kRows) * p.group - part_of_row * kCols : 0;
-        const int to = min(max(end - pos0, 0), kRows) * p.group - part_of_row * kCols;
+        const int pos0 = p.L - p.M + i * p.tile_tokens + g * p.half_tokens;      // of the half's first row; columns from .. to - 1 see the key
+        const int from = first > pos0 ? min(first - pos0, kHalf) * p.half_heads - sub * kCols : 0;
+        const int to = min(max(end - pos0, 0), kHalf) * p.half_heads - sub * kCols;
         const bool cut = __any_sync(0xffffffffu, from > 0), cut_end = __any_sync(0xffffffffu, to < kCols);
         float w[kCols];
         {
@@ -471,8 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
               const uint64_t sc2 = pack_f32x2(sc, sc), at2 = pack_f32x2(-at, -at);
 #pragma unroll
               for (int u = 0; u < 32; u += 4) {
-                const float4 sl = *reinterpret_cast<const float4*>(&rows.slope[part_of_row * kCols + u]);
-                const float4 ps = *reinterpret_cast<const float4*>(&rows.pos[part_of_row * kCols + u]);
+                const float4 sl = *reinterpret_cast<const float4*>(&rows.slope[sub * kCols + u]);
+                const float4 ps = *reinterpret_cast<const float4*>(&rows.pos[sub * kCols + u]);
 #pragma unroll
                 for (int q = 0; q < 4; q += 2) {
                   float d0, d1;
@@ -488,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
           if (mixed) {
 #pragma unroll
               for (int u = 0; u < 32; u += 4) {
-                const int4 d = *reinterpret_cast<const int4*>(&rows.doc[part_of_row * kCols + u]);
+                const int4 d = *reinterpret_cast<const int4*>(&rows.doc[sub * kCols + u]);
                 if (d.x != doc) sv[u] = __float_as_uint(-INFINITY);
                 if (d.y != doc) sv[u + 1] = __float_as_uint(-INFINITY);
                 if (d.z != doc) sv[u + 2] = __float_as_uint(-INFINITY);
@@ -512,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
 #pragma unroll
             for (int v = 0; v < 8; v += 2) {
               const int u = q * 16 + v * 2;
-              const float4 lse = *reinterpret_cast<const float4*>(&rows.lse[part_of_row * kCols + u]);
+              const float4 lse = *reinterpret_cast<const float4*>(&rows.lse[sub * kCols + u]);
               float p0, p1, p2, p3;
               unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, pack_f32x2(p_log2 - lse.x, p_log2 - lse.y), false), p0, p1);
               unpack_f32x2(softmax_weights(sv[u + 2], sv[u + 3], c2, pack_f32x2(p_log2 - lse.z, p_log2 - lse.w), weights_on_fma(u / 2 + 1)), p2, p3);
@@ -539,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
           uint32_t pk[16];
 #pragma unroll
           for (int u = 0; u < 32; u += 4) {
-            const float4 de = *reinterpret_cast<const float4*>(&rows.delta[part_of_row * kCols + u]);
+            const float4 de = *reinterpret_cast<const float4*>(&rows.delta[sub * kCols + u]);
             const int x = u;
             const float f0 = BF16 ? w[x] : w[x] * f, f1 = BF16 ? w[x + 1] : w[x + 1] * f, f2 = BF16 ? w[x + 2] : w[x + 2] * f,
                         f3 = BF16 ? w[x + 3] : w[x + 3] * f;
@@ -652,8 +663,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) sum_key_parts_kernel(const __g
 template <int D, bool BF16, bool GENERAL>
 __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __grid_constant__ BackwardParams p) {
   using LO = Layout<D>;
-  constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile;
-  constexpr uint32_t kColDp1 = 384;
+  constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile, kHalfTile = LO::kHalfTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars* bar = reinterpret_cast<Bars*>(smem + LO::kOffBar);
@@ -663,16 +673,17 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&bar->keep_full, 1);
-    mbar_init(&bar->keep_empty, 1);
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(&bar->keep_empty, 2);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bar->full[i], 1);
       mbar_init(&bar->empty[i], 2);
-      mbar_init(&bar->dp_full[i], 1);
-      mbar_init(&bar->ds_full[i], kComputeWarps);
-      mbar_init(&bar->dp_free[i], 1);
     }
-    mbar_init(&bar->s_full[0], 1);
-    mbar_init(&bar->s_taken, kComputeWarps);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&bar->s_full[g], 1);
+      mbar_init(&bar->s_taken[g], kComputeWarps / 2);
+      mbar_init(&bar->dp_full[g], 1);
+      mbar_init(&bar->ds_full[g], kComputeWarps / 2);
+    }
     mbar_init(&bar->acc_done, 1);
     mbar_init(&bar->acc_free, kComputeWarps);
     for (int i = 0; i < kSegs; ++i) {
@@ -696,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      const uint32_t tile_bytes = static_cast<uint32_t>(p.group * p.tile_tokens) * 128 * kAtoms;
+      const uint32_t half_bytes = static_cast<uint32_t>(p.half_rows) * 128 * kAtoms;
       DenseWalker<1> walker;
       Segment<1> s;
       int n = 0, keeps = 0;
@@ -717,45 +728,50 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         ok = mbar_wait(&bar->keep_empty, (keeps & 1) ^ 1, abort_word, 0x100);
         if (!ok) break;
         ++keeps;
-        mbar_arrive_expect_tx(&bar->keep_full, 2 * tile_bytes);
-        for (int a = 0; a < kAtoms; ++a) {
-          tma_load_4d(smem + LO::kOffA + a * (kRows * 128), &p.map_q, &bar->keep_full, a * 64, s.kv_head * p.group, s.first_token, s.seq);
-          tma_load_4d(smem + LO::kOffB + a * (kRows * 128), &p.map_do, &bar->keep_full, a * 64, s.kv_head * p.group, s.first_token, s.seq);
-        }
-        for (int j = s.lo0; j < s.hi0; ++j, ++n) {
-          const int st = n & 1;
-          ok = mbar_wait(&bar->empty[st], ((n >> 1) & 1) ^ 1, abort_word, 0x110);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&bar->full[st], 2 * kTile);
-          uint8_t* dst = smem + LO::kOffRing + st * 2 * kTile;
-          for (int a = 0; a < kAtoms; ++a) {
-            tma_load_4d(dst + a * (kKeys * 128), &p.map_k, &bar->full[st], a * 64, j * kKeys, s.kv_head, s.seq);
-            tma_load_4d(dst + kTile + a * (kKeys * 128), &p.map_v, &bar->full[st], a * 64, j * kKeys, s.kv_head, s.seq);
+        mbar_arrive_expect_tx(&bar->keep_full, 4 * half_bytes);
+        load_halves<D>(smem + LO::kOffA, &p.map_q, &bar->keep_full, s.kv_head * p.group, p.head_step, s.first_token, p.half_tokens, s.seq);
+        load_halves<D>(smem + LO::kOffB, &p.map_do, &bar->keep_full, s.kv_head * p.group, p.head_step, s.first_token, p.half_tokens, s.seq);
+        for (int j = s.lo0; ok && j < s.hi0; ++j, ++n) {
+          for (int g = 0; g < 2; ++g) {
+            const int h = 2 * n + g, st = h & 3;
+            ok = mbar_wait(&bar->empty[st], ((h >> 2) & 1) ^ 1, abort_word, 0x110);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&bar->full[st], kTile);
+            uint8_t* dst = smem + LO::kOffRing + st * kTile;
+            for (int a = 0; a < kAtoms; ++a) {
+              tma_load_4d(dst + a * (kHalf * 128), &p.map_k, &bar->full[st], a * 64, j * kKeys + g * kHalf, s.kv_head, s.seq);
+              tma_load_4d(dst + kHalfTile + a * (kHalf * 128), &p.map_v, &bar->full[st], a * 64, j * kKeys + g * kHalf, s.kv_head, s.seq);
+            }
           }
         }
       }
     }
   } else if (warp >= kMmaWarp) {
-    // ------------------------------------------------------------ MMA: warp 0 S = Q K^T and dP = dO V^T, warp 1 dQ += dS K
+    // ------------------------------------------------------------ MMA: warp 0 S = Q K^T, warp 1 dP = dO V^T and dQ += dS K; a block of keys in halves
     const int which = warp - kMmaWarp;
     const uint32_t issuer = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kKeys, false, false);
+    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kHalf, false, false);
     const uint32_t idesc_acc = umma_idesc_f16(BF16, kRows, D, false, true);
-    const uint64_t dq = umma_desc_sw128(smem_u32(smem + LO::kOffA), 16, 1024), ddo = umma_desc_sw128(smem_u32(smem + LO::kOffB), 16, 1024);
-    const uint64_t dk0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing), 16, 1024);
-    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing), kKeys * 128, 1024);
+    const uint64_t da = umma_desc_sw128(smem_u32(smem + (which == 0 ? LO::kOffA : LO::kOffB)), 16, 1024);
+    const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kHalfTile), 16, 1024);
+    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing), kHalf * 128, 1024);
+    const uint32_t d_first = tmem_base + (which == 0 ? kColS : kColDp);
+    uint64_t* first_full = which == 0 ? bar->s_full : bar->dp_full;
     auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
       const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
       tc_fence_after_sync();
       return r;
     };
-    auto scores = [&](uint32_t d, uint64_t a, uint64_t b) {
+    // S or dP of half g of block n: stage 2 n + g of the ring
+    auto issue_first = [&](int n, int g) {
+      const uint64_t db = db0 + ((((2 * n + g) & 3) * kTile) >> 4);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
-        umma_ss_elected(d, a + off, b + off, idesc_s, i > 0 ? 1u : 0u, issuer);
-      }
+      for (int i = 0; i < D / 16; ++i)
+        umma_ss_elected(d_first + g * kHalf, da + (((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4), db + (((i / 4) * (kHalf * 128) + (i % 4) * 32) >> 4),
+                        idesc_s, i > 0 ? 1u : 0u, issuer);
+      umma_commit_elected(&first_full[g], issuer);
     };
+    auto wait_half = [&](int n, int g) { return wait(&bar->full[(2 * n + g) & 3], (n >> 1) & 1, 0x310 + g); };
     uint32_t keeps = 0;
     int n = 0;
     bool ok = true;
@@ -766,47 +782,54 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       const int lo = segments[slot].lo0, hi = segments[slot].hi0;
       mbar_arrive_warp(&bar->seg_empty[slot], lane);
       if (lo >= hi) continue;
+      if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300))) break;
       if (which == 0) {
-        if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300))) break;
-        for (int j = lo; j < hi; ++j, ++n) {
-          const int st = n & 1;
-          const uint32_t two = (n >> 1) & 1;
-          const uint64_t dk = dk0 + ((st * 2 * kTile) >> 4);
-          if (!(ok = wait(&bar->full[st], two, 0x310) && wait(&bar->s_taken, (n & 1) ^ 1, 0x330))) break;
-          scores(tmem_base + kColS, dq, dk);
-          umma_commit_elected(&bar->s_full[0], issuer);
-          if (!(ok = wait(&bar->dp_free[st], two ^ 1, 0x331))) break;
-          scores(tmem_base + (st ? kColDp1 : kColDp), ddo, dk + (kTile >> 4));
-          umma_commit_elected(&bar->dp_full[st], issuer);
-          umma_commit_elected(&bar->empty[st], issuer);
-        }
-        umma_commit_elected(&bar->keep_empty, issuer);
+        // scores go out as soon as the last ones have been read
+        for (int j = lo; ok && j < hi; ++j, ++n)
+          for (int g = 0; g < 2; ++g) {
+            if (!(ok = wait_half(n, g) && wait(&bar->s_taken[g], (n & 1) ^ 1, 0x330))) break;
+            issue_first(n, g);
+            umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
+          }
       } else {
-        for (int j = lo; j < hi; ++j, ++n) {
-          const int st = n & 1;
-          if (j == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
-          if (!(ok = wait(&bar->ds_full[st], (n >> 1) & 1, 0x340))) break;
-          const uint64_t dr = dr0 + ((st * 2 * kTile) >> 4);
-          const uint32_t a = tmem_base + (st ? kColDp1 : kColDp);
-#pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)
-            umma_ts_elected(tmem_base + kColAcc, a + (k / 2) * kCols + (k % 2) * 8, dr + ((k * 2048) >> 4), idesc_acc, k > 0 || j > lo ? 1u : 0u, issuer);
-          umma_commit_elected(&bar->dp_free[st], issuer);
-          umma_commit_elected(&bar->empty[st], issuer);
+        for (int g = 0; g < 2; ++g) {
+          if (!(ok = ok && wait_half(n, g))) break;
+          issue_first(n, g);
         }
+        for (int j = lo; ok && j < hi; ++j, ++n)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (!(ok = ok && wait(&bar->ds_full[g], n & 1, 0x340))) break;
+            if (g == 0 && j == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
+            const uint64_t dr = dr0 + ((((2 * n + g) & 3) * kTile) >> 4);
+#pragma unroll
+            for (int q = 0; q < kHalf / 16; ++q)
+              umma_ts_elected(tmem_base + kColAcc, d_first + g * kHalf + (q / 2) * kCols + (q % 2) * 8, dr + ((q * 2048) >> 4), idesc_acc,
+                              g > 0 || q > 0 || j > lo ? 1u : 0u, issuer);
+            umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
+            if (j + 1 < hi) {
+              if (!(ok = wait_half(n + 1, g))) break;
+              issue_first(n + 1, g);
+            }
+          }
+        if (!ok) break;
         umma_commit_elected(&bar->acc_done, issuer);
       }
+      if (!ok) break;
+      umma_commit_elected(&bar->keep_empty, issuer);
       ++keeps;
     }
   } else {
     // ------------------------------------------------------------ arithmetic: thread a row and a quarter of the block's keys
-    const int quad = warp & 3, part_of_row = warp >> 2, row = quad * 32 + lane;
+    const int quad = warp & 3, part_of_row = warp >> 2, g = warp >> 3, row = quad * 32 + lane;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = p.c;
     float up, down;
     ds_scale<BF16>(p, &up, &down);
     const float p_log2 = BF16 ? 0.f : kPScaleLog2, f = BF16 ? 1.0f : up * (1.0f / 16384.0f);
-    const int r_token = row / p.group, r_head = row - r_token * p.group;
+    const int r_half = row / kHalf, r_in = row % kHalf, r_token = r_half * p.half_tokens + r_in / p.half_heads,
+              r_head = r_half * p.head_step + r_in % p.half_heads;
+    const bool row_used = r_in < p.half_rows && r_head < p.group;
     int n = 0;
     uint32_t accs = 0;
     bool ok = true;
@@ -817,9 +840,9 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       const Segment<1>& s = segments[slot];
       if (!s.valid) break;
       const int lo = s.lo0, hi = s.hi0, token = s.first_token + r_token, pos = token + s.keys - s.tokens;
-      const bool valid = r_token < p.tile_tokens && token < s.tokens;
-      const TileRows& rows = p.rows[(static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + s.first_token / p.tile_tokens];
-      const float off = p_log2 - rows.lse[row], delta = rows.delta[row], slope = GENERAL ? rows.slope[row] : 0.f;
+      const bool valid = row_used && token < s.tokens;
+      const HalfRows& rows = p.rows[((static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + s.first_token / p.tile_tokens) * 2 + r_half];
+      const float off = p_log2 - rows.lse[r_in], delta = rows.delta[r_in], slope = GENERAL ? rows.slope[r_in] : 0.f;
       int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0, low = 0, doc = -1;
       bool mixed = false;
       if (p.documents != nullptr) {
@@ -834,8 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       }
       const bool behind = p.causal && s.prefix <= s.keys - s.tokens + s.first_token + 1;      // every key that a row sees is at or in front of it
       for (int j = lo; j < hi; ++j, ++n) {
-        const int st = n & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[0], n & 1, abort_word, 0x800));
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[g], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
         const int k0 = j * kKeys + part_of_row * kCols;
@@ -891,12 +913,12 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
           }
         }
         tc_fence_before_sync();
-        mbar_arrive_warp(&bar->s_taken, lane);
+        mbar_arrive_warp(&bar->s_taken[g], lane);
 
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[st], (n >> 1) & 1, abort_word, 0x810));
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[g], n & 1, abort_word, 0x810));
         if (!ok) break;
         tc_fence_after_sync();
-        const uint32_t dp_col = lane_base + (st ? kColDp1 : kColDp) + part_of_row * kCols;
+        const uint32_t dp_col = lane_base + kColDp + part_of_row * kCols;
         {
           uint32_t dp[32], pk[16];
           tmem_ld_x32_wait(dp_col, dp);
@@ -909,7 +931,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         }
         tmem_wait_st();
         tc_fence_before_sync();
-        mbar_arrive_warp(&bar->ds_full[st], lane);
+        mbar_arrive_warp(&bar->ds_full[g], lane);
       }
       if (!ok) break;
 

@@ -5,16 +5,19 @@
 namespace ditto_b200 {
 namespace masked {
 
-// What the gradient kernels need of the 128 rows of a query tile, in the order of its rows; rows that are none have lse +infinity, which
-// makes their weights zeros.
-struct TileRows {
-  float lse[kRows];      // log2 of the sum of exponentials
-  float delta[kRows];    // sum over d of grad_out times out
-  int doc[kRows];
-  float slope[kRows];    // -slopes[head] log2(e)
-  float pos[kRows];      // position of the row's query
+// The gradient kernels take a query tile in two halves of 64 rows, each of whole tokens (64 / group of them), or, where more than 64 heads
+// share a key head, of half of one token's heads: the loads of a half go out as soon as the half of the tile before last is done with.
+constexpr int kHalf = 64;
+
+// What the gradient kernels need of a half's rows, in their order; rows that are none have lse +infinity, which makes their weights zeros.
+struct HalfRows {
+  float lse[kHalf];      // log2 of the sum of exponentials
+  float delta[kHalf];    // sum over d of grad_out times out
+  int doc[kHalf];
+  float slope[kHalf];    // -slopes[head] log2(e)
+  float pos[kHalf];      // position of the row's query
 };
-static_assert(sizeof(TileRows) == 2560, "a bulk copy of whole 16-byte pieces");
+static_assert(sizeof(HalfRows) == 1280, "a bulk copy of whole 16-byte pieces");
 
 // An item (kv head of a batch entry, block of keys) that a CTA begins and another ends.
 struct KeyPartDesc {
@@ -22,16 +25,18 @@ struct KeyPartDesc {
 };
 
 struct BackwardParams {
-  CUtensorMap map_q, map_do;  // (d, heads, tokens, batch), box 64 x group x tokens of a tile x 1
-  CUtensorMap map_k, map_v;   // (d, keys, kv heads, batch), box 64 x 128 x 1 x 1
+  CUtensorMap map_q, map_do;  // (d, heads, tokens, batch), box 64 x half_heads x half's tokens x 1
+  CUtensorMap map_k, map_v;   // (d, keys, kv heads, batch), box 64 x 64 x 1 x 1
   const void *o, *grad;       // out and its gradient, for delta
   const void* v;
   long long o_stride[3], g_stride[3], v_stride[3];      // batch, token, head; in elements
   const float* lse;           // [batch, M, heads]
   void *dq, *dk, *dv;         // contiguous
-  TileRows* rows;             // [batch][kv heads][tiles]
+  HalfRows* rows;             // [batch][kv heads][tiles][2]
   uint32_t* norms;            // largest squared norms of a row of grad_out and of v, as the bits of a float; fp16 only
   int batch, M, L, heads, kv_heads, group, tile_tokens, d, tiles, blocks;
+  // row r of half g of tile i: token i tile_tokens + g half_tokens + r / half_heads, head g head_step + r % half_heads; half_rows of them
+  int half_tokens, half_heads, head_step, half_rows;
   int items;                  // query tiles in all
   int causal;
   float c, cap_in, cap_out, score_log2, scale;
