@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid
     if (lane == 0 && at < rows) {
       HalfRows& t = p.rows[at / kHalf];
       const float lse = valid ? p.lse[(static_cast<size_t>(b) * p.M + token) * p.heads + head] : -INFINITY;
-      t.lse[r] = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
-      t.delta[r] = dot;
+      t.lse[r] = lse == -INFINITY ? -INFINITY : fmaf(lse, -1.4426950408889634f, BF16 ? 0.f : kPScaleLog2);
+      t.delta[r] = -dot;
       t.doc[r] = p.documents != nullptr && valid ? p.documents[static_cast<size_t>(b) * p.L + pos] : -1;
       t.slope[r] = p.slopes != nullptr && valid ? p.slopes[head] * -1.4426950408889634f : 0.f;
       t.pos[r] = static_cast<float>(pos);
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
     const float c = p.c;
     float up, down;
     ds_scale<BF16>(p, &up, &down);
-    const float p_log2 = BF16 ? 0.f : kPScaleLog2, p_down = BF16 ? 1.0f : 1.0f / 16384.0f;
+    const float p_down = BF16 ? 1.0f : 1.0f / 16384.0f;
     const float f = BF16 ? 1.0f : up * p_down;
     int n = 0;
     uint32_t accs = 0;
@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         }
         mixed = p.mixed[s.seq] != 0;
       }
+      const int first_of_all = __reduce_max_sync(0xffffffffu, first), end_of_all = __reduce_min_sync(0xffffffffu, end);
       for (int i = lo; i < hi; ++i, ++n) {
         const int st = (2 * n + g) & 3;
         const HalfRows& rows = *reinterpret_cast<const HalfRows*>(smem + LO::kOffRows + st * sizeof(HalfRows));
@@ -453,10 +454,10 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         if (!ok) break;
         tc_fence_after_sync();
         const int pos0 = p.L - p.M + i * p.tile_tokens + g * p.half_tokens;      // of the half's first row; columns from .. to - 1 see the key
+        const bool cut = first_of_all > pos0, cut_end = end_of_all < pos0 + kHalf;      // (a half has at most that many tokens)
         const int from = first > pos0 ? min(first - pos0, kHalf) * p.half_heads - sub * kCols : 0;
         const int to = min(max(end - pos0, 0), kHalf) * p.half_heads - sub * kCols;
-        const bool cut = __any_sync(0xffffffffu, from > 0), cut_end = __any_sync(0xffffffffu, to < kCols);
-        float w[kCols];
+        float w[kCols] = {};
         {
           uint32_t sv[32];
           tmem_ld_x32_wait(s_col, sv);
@@ -473,9 +474,6 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
                 unpack_f32x2(mul_f32x2(t, out2), y0, y1);
                 sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
-            } else {
-#pragma unroll
-              for (int u = 0; u < 32; ++u) w[u] = 1.0f;
             }
             if (p.slopes != nullptr) {
               const float sc = p.cap_out != 0.f ? 1.0f : p.score_log2, at = static_cast<float>(key);
@@ -524,14 +522,18 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
             for (int v = 0; v < 8; v += 2) {
               const int u = q * 16 + v * 2;
               const float4 lse = *reinterpret_cast<const float4*>(&rows.lse[sub * kCols + u]);
+              const uint64_t p01 = softmax_weights(sv[u], sv[u + 1], c2, pack_f32x2(lse.x, lse.y), false);
+              const uint64_t p23 = softmax_weights(sv[u + 2], sv[u + 3], c2, pack_f32x2(lse.z, lse.w), weights_on_fma(u / 2 + 1));
               float p0, p1, p2, p3;
-              unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, pack_f32x2(p_log2 - lse.x, p_log2 - lse.y), false), p0, p1);
-              unpack_f32x2(softmax_weights(sv[u + 2], sv[u + 3], c2, pack_f32x2(p_log2 - lse.z, p_log2 - lse.w), weights_on_fma(u / 2 + 1)), p2, p3);
+              unpack_f32x2(p01, p0, p1);
+              unpack_f32x2(p23, p2, p3);
               pk[v] = pack2<BF16>(p0, p1);
               pk[v + 1] = pack2<BF16>(p2, p3);
-              const int x = u;
-              w[x] = GENERAL ? p0 * w[x] : p0, w[x + 1] = GENERAL ? p1 * w[x + 1] : p1;
-              w[x + 2] = GENERAL ? p2 * w[x + 2] : p2, w[x + 3] = GENERAL ? p3 * w[x + 3] : p3;
+              uint64_t w01 = p01, w23 = p23;
+              if (GENERAL && p.cap_out != 0.f) w01 = mul_f32x2(w01, pack_f32x2(w[u], w[u + 1])), w23 = mul_f32x2(w23, pack_f32x2(w[u + 2], w[u + 3]));
+              if constexpr (!BF16) w01 = mul_f32x2(w01, pack_f32x2(f, f)), w23 = mul_f32x2(w23, pack_f32x2(f, f));
+              unpack_f32x2(w01, w[u], w[u + 1]);
+              unpack_f32x2(w23, w[u + 2], w[u + 3]);
             }
             // (packed weights go over the first half of this thread's own columns)
             tmem_st_x8(s_col + q * 8, pk);
@@ -551,11 +553,13 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
 #pragma unroll
           for (int u = 0; u < 32; u += 4) {
             const float4 de = *reinterpret_cast<const float4*>(&rows.delta[sub * kCols + u]);
-            const int x = u;
-            const float f0 = BF16 ? w[x] : w[x] * f, f1 = BF16 ? w[x + 1] : w[x + 1] * f, f2 = BF16 ? w[x + 2] : w[x + 2] * f,
-                        f3 = BF16 ? w[x + 3] : w[x + 3] * f;
-            pk[u / 2] = pack2<BF16>(f0 * (__uint_as_float(dp[u]) - de.x), f1 * (__uint_as_float(dp[u + 1]) - de.y));
-            pk[u / 2 + 1] = pack2<BF16>(f2 * (__uint_as_float(dp[u + 2]) - de.z), f3 * (__uint_as_float(dp[u + 3]) - de.w));
+            auto product = [&](int i, float d0, float d1) {
+              float x0, x1;
+              unpack_f32x2(mul_f32x2(pack_f32x2(w[i], w[i + 1]), add_f32x2(pack_f32x2(__uint_as_float(dp[i]), __uint_as_float(dp[i + 1])), pack_f32x2(d0, d1))), x0, x1);
+              return pack2<BF16>(x0, x1);
+            };
+            pk[u / 2] = product(u, de.x, de.y);
+            pk[u / 2 + 1] = product(u + 2, de.z, de.w);
           }
           tmem_st_x16(dp_col, pk);
         }
@@ -826,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
     const float c = p.c;
     float up, down;
     ds_scale<BF16>(p, &up, &down);
-    const float p_log2 = BF16 ? 0.f : kPScaleLog2, f = BF16 ? 1.0f : up * (1.0f / 16384.0f);
+    const float f = BF16 ? 1.0f : up * (1.0f / 16384.0f);
     const int r_half = row / kHalf, r_in = row % kHalf, r_token = r_half * p.half_tokens + r_in / p.half_heads,
               r_head = r_half * p.head_step + r_in % p.half_heads;
     const bool row_used = r_in < p.half_rows && r_head < p.group;
@@ -842,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       const int lo = s.lo0, hi = s.hi0, token = s.first_token + r_token, pos = token + s.keys - s.tokens;
       const bool valid = row_used && token < s.tokens;
       const HalfRows& rows = p.rows[((static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + s.first_token / p.tile_tokens) * 2 + r_half];
-      const float off = p_log2 - rows.lse[r_in], delta = rows.delta[r_in], slope = GENERAL ? rows.slope[r_in] : 0.f;
+      const float off = rows.lse[r_in], delta = rows.delta[r_in], slope = GENERAL ? rows.slope[r_in] : 0.f;
       int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0, low = 0, doc = -1;
       bool mixed = false;
       if (p.documents != nullptr) {
@@ -855,14 +859,15 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         }
         mixed = p.mixed[s.seq] != 0;
       }
+      const int limit_of_all = __reduce_min_sync(0xffffffffu, limit), low_of_all = __reduce_max_sync(0xffffffffu, low);
       const bool behind = p.causal && s.prefix <= s.keys - s.tokens + s.first_token + 1;      // every key that a row sees is at or in front of it
       for (int j = lo; j < hi; ++j, ++n) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[g], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
         const int k0 = j * kKeys + part_of_row * kCols;
-        const bool cut = __any_sync(0xffffffffu, limit < k0 + kCols), cut_low = __any_sync(0xffffffffu, low > k0);
-        float w[kCols];
+        const bool cut = limit_of_all < k0 + kCols, cut_low = low_of_all > k0;
+        float w[kCols] = {};
         {
           uint32_t sv[32];
           tmem_ld_x32_wait(lane_base + kColS + part_of_row * kCols, sv);
@@ -878,9 +883,6 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
                 unpack_f32x2(mul_f32x2(t, out2), y0, y1);
                 sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
-            } else {
-#pragma unroll
-              for (int u = 0; u < 32; ++u) w[u] = 1.0f;
             }
             if (p.slopes != nullptr) biased(sv, p.cap_out != 0.f ? 1.0f : p.score_log2, -slope, static_cast<float>(pos - k0), behind);
           }
@@ -906,10 +908,10 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
           const uint64_t c2 = pack_f32x2(c, c), off2 = pack_f32x2(off, off);
 #pragma unroll
           for (int u = 0; u < 32; u += 2) {
-            float p0, p1;
-            unpack_f32x2(softmax_weights(sv[u], sv[u + 1], c2, off2, weights_on_fma(u / 2)), p0, p1);
-            w[u] = GENERAL ? p0 * w[u] : p0;
-            w[u + 1] = GENERAL ? p1 * w[u + 1] : p1;
+            uint64_t x = softmax_weights(sv[u], sv[u + 1], c2, off2, weights_on_fma(u / 2));
+            if (GENERAL && p.cap_out != 0.f) x = mul_f32x2(x, pack_f32x2(w[u], w[u + 1]));
+            if constexpr (!BF16) x = mul_f32x2(x, pack_f32x2(f, f));
+            unpack_f32x2(x, w[u], w[u + 1]);
           }
         }
         tc_fence_before_sync();
@@ -920,12 +922,14 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         tc_fence_after_sync();
         const uint32_t dp_col = lane_base + kColDp + part_of_row * kCols;
         {
+          const uint64_t delta2 = pack_f32x2(delta, delta);
           uint32_t dp[32], pk[16];
           tmem_ld_x32_wait(dp_col, dp);
 #pragma unroll
           for (int u = 0; u < 32; u += 2) {
-            const float w0 = BF16 ? w[u] : w[u] * f, w1 = BF16 ? w[u + 1] : w[u + 1] * f;
-            pk[u / 2] = pack2<BF16>(w0 * (__uint_as_float(dp[u]) - delta), w1 * (__uint_as_float(dp[u + 1]) - delta));
+            float x0, x1;
+            unpack_f32x2(mul_f32x2(pack_f32x2(w[u], w[u + 1]), add_f32x2(pack_f32x2(__uint_as_float(dp[u]), __uint_as_float(dp[u + 1])), delta2)), x0, x1);
+            pk[u / 2] = pack2<BF16>(x0, x1);
           }
           tmem_st_x16(dp_col, pk);
         }

@@ -9,10 +9,10 @@ namespace masked {
 // share a key head, of half of one token's heads: the loads of a half go out as soon as the half of the tile before last is done with.
 constexpr int kHalf = 64;
 
-// What the gradient kernels need of a half's rows, in their order; rows that are none have lse +infinity, which makes their weights zeros.
+// What the gradient kernels need of a half's rows, in their order; rows that are none have -infinity for lse, which makes their weights zeros.
 struct HalfRows {
-  float lse[kHalf];      // log2 of the sum of exponentials
-  float delta[kHalf];    // sum over d of grad_out times out
+  float lse[kHalf];      // -log2 of the sum of exponentials (negative: what is added to an exponent)
+  float delta[kHalf];    // -sum over d of grad_out times out
   int doc[kHalf];
   float slope[kHalf];    // -slopes[head] log2(e)
   float pos[kHalf];      // position of the row's query
