@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const uint64_t dr = dr0 + ((((2 * n + g) & 3) * kTile) >> 4);
+          if (i + 1 < hi && !(ok = ok && wait_half(n + 1, g))) break;      // (there long before its turn)
           if (!(ok = ok && wait(&back_full[g], n & 1, 0x340 + which))) break;
           if (g == 0 && i == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
 #pragma unroll
@@ -398,10 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
             umma_ts_elected(d_acc, d_first + g * kHalf + (q / 2) * kCols + (q % 2) * 8, dr + ((q * 2048) >> 4), idesc_acc,
                             g > 0 || q > 0 || i > lo ? 1u : 0u, issuer);
           umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
-          if (i + 1 < hi) {
-            if (!(ok = wait_half(n + 1, g))) break;
-            issue_first(n + 1, g);
-          }
+          if (i + 1 < hi) issue_first(n + 1, g);
         }
         if (!ok) break;
       }
@@ -455,8 +453,6 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
         tc_fence_after_sync();
         const int pos0 = p.L - p.M + i * p.tile_tokens + g * p.half_tokens;      // of the half's first row; columns from .. to - 1 see the key
         const bool cut = first_of_all > pos0, cut_end = end_of_all < pos0 + kHalf;      // (a half has at most that many tokens)
-        const int from = first > pos0 ? min(first - pos0, kHalf) * p.half_heads - sub * kCols : 0;
-        const int to = min(max(end - pos0, 0), kHalf) * p.half_heads - sub * kCols;
         float w[kCols] = {};
         {
           uint32_t sv[32];
@@ -505,11 +501,13 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
               }
           }
           if (cut) {
+            const int from = first > pos0 ? min(first - pos0, kHalf) * p.half_heads - sub * kCols : 0;
 #pragma unroll
             for (int u = 0; u < 32; ++u)
               if (u < from) sv[u] = __float_as_uint(-INFINITY);
           }
           if (cut_end) {
+            const int to = min(max(end - pos0, 0), kHalf) * p.half_heads - sub * kCols;
 #pragma unroll
             for (int u = 0; u < 32; ++u)
               if (u >= to) sv[u] = __float_as_uint(-INFINITY);
@@ -523,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
               const int u = q * 16 + v * 2;
               const float4 lse = *reinterpret_cast<const float4*>(&rows.lse[sub * kCols + u]);
               const uint64_t p01 = softmax_weights(sv[u], sv[u + 1], c2, pack_f32x2(lse.x, lse.y), false);
-              const uint64_t p23 = softmax_weights(sv[u + 2], sv[u + 3], c2, pack_f32x2(lse.z, lse.w), weights_on_fma(u / 2 + 1));
+              const uint64_t p23 = softmax_weights(sv[u + 2], sv[u + 3], c2, pack_f32x2(lse.z, lse.w), false);
               float p0, p1, p2, p3;
               unpack_f32x2(p01, p0, p1);
               unpack_f32x2(p23, p2, p3);
@@ -803,6 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         for (int j = lo; ok && j < hi; ++j, ++n)
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
+            if (j + 1 < hi && !(ok = ok && wait_half(n + 1, g))) break;
             if (!(ok = ok && wait(&bar->ds_full[g], n & 1, 0x340))) break;
             if (g == 0 && j == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
             const uint64_t dr = dr0 + ((((2 * n + g) & 3) * kTile) >> 4);
@@ -811,10 +810,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
               umma_ts_elected(tmem_base + kColAcc, d_first + g * kHalf + (q / 2) * kCols + (q % 2) * 8, dr + ((q * 2048) >> 4), idesc_acc,
                               g > 0 || q > 0 || j > lo ? 1u : 0u, issuer);
             umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
-            if (j + 1 < hi) {
-              if (!(ok = wait_half(n + 1, g))) break;
-              issue_first(n + 1, g);
-            }
+            if (j + 1 < hi) issue_first(n + 1, g);
           }
         if (!ok) break;
         umma_commit_elected(&bar->acc_done, issuer);
@@ -908,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
           const uint64_t c2 = pack_f32x2(c, c), off2 = pack_f32x2(off, off);
 #pragma unroll
           for (int u = 0; u < 32; u += 2) {
-            uint64_t x = softmax_weights(sv[u], sv[u + 1], c2, off2, weights_on_fma(u / 2));
+            uint64_t x = softmax_weights(sv[u], sv[u + 1], c2, off2, false);
             if (GENERAL && p.cap_out != 0.f) x = mul_f32x2(x, pack_f32x2(w[u], w[u + 1]));
             if constexpr (!BF16) x = mul_f32x2(x, pack_f32x2(f, f));
             unpack_f32x2(x, w[u], w[u + 1]);
