@@ -73,57 +73,69 @@ __device__ __forceinline__ void dot8(uint4 a, uint4 b, float& dot, float& norm_a
   }
 }
 
-// Half a warp a row.  Bound by reading out and its gradient once.
-template <bool BF16>
+// A CTA half a tile at a time, LANES threads a row of it and kRowsAtOnce rows in flight a thread.  Bound by reading out and its gradient once.
+template <bool BF16, int LANES>
 __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid_constant__ BackwardParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int lane = threadIdx.x & 15, pieces = p.d / 8;
-  const long long rows = static_cast<long long>(p.batch) * p.kv_heads * p.tiles * kRows, step = static_cast<long long>(gridDim.x) * (kRowThreads / 16);
+  constexpr int kSpan = kRowThreads / LANES, kRowsAtOnce = kHalf / kSpan;
+  const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES, pieces = p.d / 8;
+  const int halves = p.items * 2;
   float norm_g = 0.f, norm_v = 0.f;
-  // (the loops' bounds are those of whole warps: shuffles)
-  for (long long at = static_cast<long long>(blockIdx.x) * (kRowThreads / 16) + threadIdx.x / 16; at - (threadIdx.x / 16 & 1) < rows; at += step) {
-    const int r = static_cast<int>(at % kHalf), g = static_cast<int>(at / kHalf % 2);
-    long long rest = at / kRows;
-    const int tile = static_cast<int>(rest % p.tiles);
-    rest /= p.tiles;
-    const int kv_head = static_cast<int>(rest % p.kv_heads), b = static_cast<int>(rest / p.kv_heads);
-    const int token = tile * p.tile_tokens + g * p.half_tokens + r / p.half_heads, in_group = g * p.head_step + r % p.half_heads;
-    const int head = kv_head * p.group + in_group, pos = token + p.L - p.M;
-    const bool valid = at < rows && r < p.half_rows && in_group < p.group && token < p.M;
-    float dot = 0.f, norm = 0.f;
-    if (valid && lane < pieces) {
-      const uint4 g = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.grad) + 2 * (b * p.g_stride[0] + token * p.g_stride[1] + head * p.g_stride[2]) + lane * 16);
-      const uint4 o = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.o) + 2 * (b * p.o_stride[0] + token * p.o_stride[1] + head * p.o_stride[2]) + lane * 16);
-      dot8<BF16>(g, o, dot, norm);
-    }
+  for (int at = blockIdx.x; at < halves; at += gridDim.x) {
+    const int g = at & 1, tile = at / 2 % p.tiles, kv_head = at / 2 / p.tiles % p.kv_heads, b = at / 2 / p.tiles / p.kv_heads;
+    const int token0 = tile * p.tile_tokens + g * p.half_tokens;
+    uint4 vg[kRowsAtOnce], vo[kRowsAtOnce];
+    int token[kRowsAtOnce], head[kRowsAtOnce];
+    bool valid[kRowsAtOnce];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      norm += __shfl_xor_sync(0xffffffffu, norm, o);
+    for (int i = 0; i < kRowsAtOnce; ++i) {
+      const int r = first + i * kSpan, of_half = r / p.half_heads, in_group = g * p.head_step + r - of_half * p.half_heads;
+      token[i] = token0 + of_half;
+      head[i] = kv_head * p.group + in_group;
+      valid[i] = r < p.half_rows && in_group < p.group && token[i] < p.M;
+      vg[i] = vo[i] = make_uint4(0, 0, 0, 0);
+      if (valid[i] && lane < pieces) {
+        vg[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.grad) + 2 * (b * p.g_stride[0] + token[i] * p.g_stride[1] + head[i] * p.g_stride[2]) + lane * 16);
+        vo[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.o) + 2 * (b * p.o_stride[0] + token[i] * p.o_stride[1] + head[i] * p.o_stride[2]) + lane * 16);
+      }
     }
-    norm_g = fmaxf(norm_g, norm);
-    if (lane == 0 && at < rows) {
-      HalfRows& t = p.rows[at / kHalf];
-      const float lse = valid ? p.lse[(static_cast<size_t>(b) * p.M + token) * p.heads + head] : -INFINITY;
-      t.lse[r] = lse == -INFINITY ? -INFINITY : fmaf(lse, -1.4426950408889634f, BF16 ? 0.f : kPScaleLog2);
-      t.delta[r] = -dot;
-      t.doc[r] = p.documents != nullptr && valid ? p.documents[static_cast<size_t>(b) * p.L + pos] : -1;
-      t.slope[r] = p.slopes != nullptr && valid ? p.slopes[head] * -1.4426950408889634f : 0.f;
-      t.pos[r] = static_cast<float>(pos);
+    HalfRows& t = p.rows[at];
+#pragma unroll
+    for (int i = 0; i < kRowsAtOnce; ++i) {
+      float dot = 0.f, norm = 0.f;
+      dot8<BF16>(vg[i], vo[i], dot, norm);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) {
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (!BF16) norm += __shfl_xor_sync(0xffffffffu, norm, o);
+      }
+      norm_g = fmaxf(norm_g, norm);
+      if (lane == 0) {
+        const int r = first + i * kSpan, pos = token[i] + p.L - p.M;
+        const float lse = valid[i] ? p.lse[(static_cast<size_t>(b) * p.M + token[i]) * p.heads + head[i]] : -INFINITY;
+        t.lse[r] = lse == -INFINITY ? -INFINITY : fmaf(lse, -1.4426950408889634f, BF16 ? 0.f : kPScaleLog2);
+        t.delta[r] = -dot;
+        t.doc[r] = p.documents != nullptr && valid[i] ? p.documents[static_cast<size_t>(b) * p.L + pos] : -1;
+        t.slope[r] = p.slopes != nullptr && valid[i] ? p.slopes[head[i]] * -1.4426950408889634f : 0.f;
+        t.pos[r] = static_cast<float>(pos);
+      }
     }
   }
   if constexpr (!BF16) {
-    const long long keys = static_cast<long long>(p.batch) * p.L * p.kv_heads;
-    for (long long at = static_cast<long long>(blockIdx.x) * (kRowThreads / 16) + threadIdx.x / 16; at - (threadIdx.x / 16 & 1) < keys; at += step) {
-      const int h = static_cast<int>(at % p.kv_heads), j = static_cast<int>(at / p.kv_heads % p.L), b = static_cast<int>(at / p.kv_heads / p.L);
+    // (the loop's bounds are those of whole warps: shuffles)
+    constexpr int kPerWarp = 32 / LANES;
+    const long long keys = static_cast<long long>(p.batch) * p.L * p.kv_heads, step = static_cast<long long>(gridDim.x) * kSpan;
+    for (long long at = static_cast<long long>(blockIdx.x) * kSpan + first; at - first % kPerWarp < keys; at += step) {
+      const long long of_head = at / p.kv_heads;
+      const int h = static_cast<int>(at - of_head * p.kv_heads), b = static_cast<int>(of_head / p.L), j = static_cast<int>(of_head - static_cast<long long>(b) * p.L);
       float dot = 0.f, norm = 0.f;
       if (at < keys && lane < pieces) {
         const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.v) + 2 * (b * p.v_stride[0] + j * p.v_stride[1] + h * p.v_stride[2]) + lane * 16);
         dot8<BF16>(v, v, dot, norm);
       }
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, o);
+      for (int o = LANES / 2; o > 0; o >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, o);
       norm_v = fmaxf(norm_v, norm);
     }
     // the largest of all: the order of atomics does not show in it
@@ -630,10 +642,11 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
 
 namespace {
 
-// Sums of the parts of a block that several CTAs had, in the order of its tiles.  One CTA for the block that CTA blockIdx.x began.
-constexpr int kSumThreads = 512;
+// Sums of the parts of a block that several CTAs had, in the order of its tiles.  CTAs (x, ..) for the block that CTA x of the kernel above
+// began, kSumSlices of them with 1 / kSumSlices of its values each.
+constexpr int kSumThreads = 256, kSumSlices = 8;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kSumThreads, 1) sum_key_parts_kernel(const __grid_constant__ BackwardParams p) {
+__global__ void __launch_bounds__(kSumThreads) sum_key_parts_kernel(const __grid_constant__ BackwardParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const KeyPartDesc part = p.parts[blockIdx.x];
@@ -641,7 +654,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) sum_key_parts_kernel(const __g
   const int block = part.item % p.blocks, kv_head = part.item / p.blocks % p.kv_heads, seq = part.item / p.blocks / p.kv_heads;
   float up, down;
   ds_scale<BF16>(p, &up, &down);
-  for (int i = threadIdx.x; i < 2 * kKeys * (D / 8); i += kSumThreads) {
+  for (int i = blockIdx.y * kSumThreads + threadIdx.x; i < 2 * kKeys * (D / 8); i += kSumThreads * kSumSlices) {
     const int col = i % (D / 8) * 8, row = i / (D / 8) % kKeys, m = i / (D / 8) / kKeys, key = block * kKeys + row;
     if (key >= p.L || col >= p.d) continue;
     float x[8] = {};
@@ -984,9 +997,9 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
 
 namespace {
 
-cudaLaunchConfig_t config(long long grid, int threads, int smem, cudaStream_t stream, cudaLaunchAttribute* attr) {
+cudaLaunchConfig_t config(long long grid, int threads, int smem, cudaStream_t stream, cudaLaunchAttribute* attr, int slices = 1) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), static_cast<unsigned>(slices), 1);
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
@@ -1013,7 +1026,7 @@ cudaError_t launch_products(const BackwardParams& p, int sms, cudaStream_t strea
   }
   cudaLaunchAttribute attr[1];
   e = launch_kernel(config(sms, kThreads, Layout<D>::kBytes, stream, attr), keys, p);
-  if (e == cudaSuccess) e = launch_kernel(config(sms, kSumThreads, 0, stream, attr), sum_key_parts_kernel<D, BF16>, p);
+  if (e == cudaSuccess) e = launch_kernel(config(sms, kSumThreads, 0, stream, attr, kSumSlices), sum_key_parts_kernel<D, BF16>, p);
   if (e == cudaSuccess) e = launch_kernel(config(p.items < sms ? p.items : sms, kThreads, Layout<D>::kBytes, stream, attr), queries, p);
   return e;
 }
@@ -1026,9 +1039,9 @@ cudaError_t launch_backward(const BackwardParams& p, int sms, cudaStream_t strea
     const cudaError_t e = cudaMemsetAsync(p.norms, 0, 2 * sizeof(uint32_t), stream);
     if (e != cudaSuccess) return e;
   }
-  const long long rows = static_cast<long long>(p.batch) * p.kv_heads * p.tiles * kRows, ctas = (rows + kRowThreads / 16 - 1) / (kRowThreads / 16);
   cudaLaunchAttribute attr[1];
-  const cudaError_t e = launch_kernel(config(ctas < 8 * sms ? ctas : 8 * sms, kRowThreads, 0, stream, attr), backward_rows_kernel<BF16>, p);
+  const cudaLaunchConfig_t rows = config(2 * p.items < 8 * sms ? 2 * p.items : 8 * sms, kRowThreads, 0, stream, attr);
+  const cudaError_t e = D == 64 ? launch_kernel(rows, backward_rows_kernel<BF16, 8>, p) : launch_kernel(rows, backward_rows_kernel<BF16, 16>, p);
   if (e != cudaSuccess) return e;
   const bool general = p.cap_out != 0.f || p.slopes != nullptr;
   return general ? launch_products<D, BF16, true>(p, sms, stream) : launch_products<D, BF16, false>(p, sms, stream);

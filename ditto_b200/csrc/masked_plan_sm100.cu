@@ -60,29 +60,61 @@ __global__ void __launch_bounds__(kPlanThreads, 1) document_plan_kernel(const in
   // Runs of equal ids: a position's run begins at the last change of id up to it and ends at the first one behind it.  They are its document
   // where every id has one run, which is certain where the ids rise.
   int2* my_runs = runs + static_cast<size_t>(b) * L;
+  constexpr int kEach = 4;                             // positions of a thread, one behind the other
   int begin = 0, highest = -1;
   bool falls = false;
-  for (int base = 0; base < L; base += kPlanThreads) {
-    const int k = base + static_cast<int>(threadIdx.x), id = k < L ? ids[k] : -1;
-    const bool change = k < L && (k == 0 || ids[k - 1] != id);
-    int before, all;
-    const int at = max(begin, block_max(change ? k : 0, 0, scratch, &before, &all));
+  for (int base = 0; base < L; base += kPlanThreads * kEach) {
+    const int k0 = base + static_cast<int>(threadIdx.x) * kEach;
+    int last = k0 > 0 && k0 <= L ? ids[k0 - 1] : -1, change[kEach], id[kEach], latest = 0, most = -1, before, all;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int k = k0 + u;
+      id[u] = k < L ? ids[k] : -1;
+      change[u] = k < L && (k == 0 || id[u] != last);
+      if (change[u]) latest = k;
+      last = id[u];
+      most = max(most, id[u]);
+    }
+    block_max(latest, 0, scratch, &before, &all);
+    int at = max(begin, before);
     begin = max(begin, all);
-    block_max(id, -1, scratch, &before, &all);
-    falls |= change && id >= 0 && id <= max(highest, before);
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      if (change[u]) at = k0 + u;
+      if (k0 + u < L) my_runs[k0 + u].x = at;
+    }
+    block_max(most, -1, scratch, &before, &all);
+    int up_to = max(highest, before);
     highest = max(highest, all);
-    if (k < L) my_runs[k].x = at;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      falls |= change[u] && id[u] >= 0 && id[u] <= up_to;
+      up_to = max(up_to, id[u]);
+    }
   }
   const bool any_order = __syncthreads_or(falls);
   if (threadIdx.x == 0) mixed[b] = any_order;
   int end = 0;                                         // (of the positions counted from the row's end)
-  for (int base = 0; base < L; base += kPlanThreads) {
-    const int r = base + static_cast<int>(threadIdx.x), k = L - 1 - r, id = r < L ? ids[k] : -1;
-    const bool change = r < L && (r == 0 || ids[k + 1] != id);
-    int before, all;
-    const int at = max(end, block_max(change ? r : 0, 0, scratch, &before, &all));
+  for (int base = 0; base < L; base += kPlanThreads * kEach) {
+    const int r0 = base + static_cast<int>(threadIdx.x) * kEach;
+    int last = r0 > 0 && r0 <= L ? ids[L - r0] : -1, change[kEach], id[kEach], latest = 0, before, all;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int r = r0 + u;
+      id[u] = r < L ? ids[L - 1 - r] : -1;
+      change[u] = r < L && (r == 0 || id[u] != last);
+      if (change[u]) latest = r;
+      last = id[u];
+    }
+    block_max(latest, 0, scratch, &before, &all);
+    int at = max(end, before);
     end = max(end, all);
-    if (r < L) my_runs[k] = id < 0 ? make_int2(0, 0) : any_order ? make_int2(0, L) : make_int2(my_runs[k].x, L - at);
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int r = r0 + u, k = L - 1 - r;
+      if (change[u]) at = r;
+      if (r < L) my_runs[k] = id[u] < 0 ? make_int2(0, 0) : any_order ? make_int2(0, L) : make_int2(my_runs[k].x, L - at);
+    }
   }
   for (int j = warp; j < blocks; j += warps) {
     int least = INT_MAX, most = -1;
@@ -130,11 +162,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) document_plan_kernel(const in
   }
 }
 
-// Sum of an item's parts, in the order of its keys: O = sum_p 2^(c (m_p - m)) O_p / sum_p 2^(c (m_p - m)) l_p.  One CTA for the item that
-// CTA blockIdx.x of the forward kernel began; a warp a row.
-constexpr int kSumThreads = 512;
+// Sum of an item's parts, in the order of its keys: O = sum_p 2^(c (m_p - m)) O_p / sum_p 2^(c (m_p - m)) l_p.  CTAs (x, ..) for the item that
+// CTA x of the forward kernel began, a warp a row.
+constexpr int kSumThreads = 256, kSumSlices = 8;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kSumThreads, 1) sum_parts_kernel(const __grid_constant__ Params p, const int rows) {
+__global__ void __launch_bounds__(kSumThreads) sum_parts_kernel(const __grid_constant__ Params p, const int rows) {
   grid_dependency_wait();
   grid_launch_dependents();
   const PartDesc part = p.parts[blockIdx.x];
@@ -142,7 +174,7 @@ __global__ void __launch_bounds__(kSumThreads, 1) sum_parts_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = part.last_cta - static_cast<int>(blockIdx.x) + 1;
   Sequence q;
   q.load(p, part.seq);
-  for (int r = warp; r < rows; r += kSumThreads / 32) {
+  for (int r = blockIdx.y + kSumSlices * warp; r < rows; r += kSumSlices * (kSumThreads / 32)) {
     const int in_tile = r % kRows, token = part.first_token + (r / kRows) * p.tile_tokens + in_tile / p.group;
     if (in_tile / p.group >= p.tile_tokens || token >= q.tokens) continue;
     auto at = [&](int i) { return (static_cast<size_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * rows + r; };
@@ -181,9 +213,9 @@ __global__ void __launch_bounds__(kSumThreads, 1) sum_parts_kernel(const __grid_
   }
 }
 
-cudaLaunchConfig_t config(int grid, int threads, cudaStream_t stream, cudaLaunchAttribute* attr) {
+cudaLaunchConfig_t config(int grid, int threads, cudaStream_t stream, cudaLaunchAttribute* attr, int slices = 1) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), static_cast<unsigned>(slices), 1);
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -205,7 +237,7 @@ cudaError_t launch_document_plan(const int* documents, const int* prefix, int ba
 
 cudaError_t launch_sum_parts(const Params& p, int d, bool bf16, int tiles, int grid, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = config(grid, kSumThreads, stream, attr);
+  const cudaLaunchConfig_t cfg = config(grid, kSumThreads, stream, attr, kSumSlices);
   const int rows = tiles * kRows;
   if (d == 128) return bf16 ? launch_kernel(cfg, sum_parts_kernel<128, true>, p, rows) : launch_kernel(cfg, sum_parts_kernel<128, false>, p, rows);
   return bf16 ? launch_kernel(cfg, sum_parts_kernel<64, true>, p, rows) : launch_kernel(cfg, sum_parts_kernel<64, false>, p, rows);
