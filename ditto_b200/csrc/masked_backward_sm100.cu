@@ -172,7 +172,7 @@ struct Layout {
 struct Bars {
   uint64_t keep_full, keep_empty;
   uint64_t full[4], empty[4];
-  uint64_t s_full[2], s_taken[2], p_full[2], dp_full[2], ds_full[2], acc_done, acc_free;
+  uint64_t s_full[2], p_full[2], dp_full[2], ds_full[2], acc_done, acc_free;
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   uint32_t tmem_base, abort_word;
   int start_item, start_tile, left, per_cta;
@@ -246,10 +246,83 @@ __device__ __forceinline__ void load_halves(uint8_t* dst, const CUtensorMap* map
     for (int g = 0; g < 2; ++g) tma_load_4d(dst + a * (kRows * 128) + g * (kHalf * 128), map, bar, a * 64, x1 + g * x1_step, x2 + g * x2_step, x3);
 }
 
+// What the two MMA warps of either kernel do (a converged warp, an elected lane issues).  Warp 0: scores S of what stays at kOffA with the
+// first operand of a stage, and the first sum, from P; warp 1: dP of what stays at kOffB with the second operand, and the second sum, from dS.
+// Both sums' other operand is an operand of the stage too, its rows as the reduction: `sum_of` says which, 0 or 1.  What
+// stays has 128 rows, a stage holds half of the 128 that pass: the halves have score columns of their own, so that one's products run
+// under the other's arithmetic.  `range` gives the tiles or blocks of a segment.
+template <int D, bool BF16, class Seg, class Range>
+__device__ __forceinline__ void issue_products(uint8_t* smem, Bars* bar, uint32_t tmem_base, const Seg* segments, int which, int lane, int sum_of,
+                                               Range range) {
+  using LO = Layout<D>;
+  constexpr int kTile = LO::kTile, kHalfTile = LO::kHalfTile;
+  volatile uint32_t* abort_word = &bar->abort_word;
+  const uint32_t issuer = elect_one();
+  const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kHalf, false, false);
+  const uint32_t idesc_acc = umma_idesc_f16(BF16, kRows, D, false, true);
+  const uint64_t da = umma_desc_sw128(smem_u32(smem + (which == 0 ? LO::kOffA : LO::kOffB)), 16, 1024);
+  const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kHalfTile), 16, 1024);
+  const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + sum_of * kHalfTile), kHalf * 128, 1024);
+  const uint32_t d_first = tmem_base + (which == 0 ? kColS : kColDp), d_acc = tmem_base + kColAcc + which * D;
+  uint64_t* first_full = which == 0 ? bar->s_full : bar->dp_full;
+  uint64_t* back_full = which == 0 ? bar->p_full : bar->ds_full;
+  auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
+    const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
+    tc_fence_after_sync();
+    return r;
+  };
+  // the scores of half g of tile or block n: stage 2 n + g of the ring
+  auto issue_first = [&](int n, int g) {
+    const uint64_t db = db0 + ((((2 * n + g) & 3) * kTile) >> 4);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      umma_ss_elected(d_first + g * kHalf, da + (((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4), db + (((i / 4) * (kHalf * 128) + (i % 4) * 32) >> 4),
+                      idesc_s, i > 0 ? 1u : 0u, issuer);
+    umma_commit_elected(&first_full[g], issuer);
+  };
+  auto wait_half = [&](int n, int g) { return wait(&bar->full[(2 * n + g) & 3], (n >> 1) & 1, 0x310 + g); };
+  uint32_t keeps = 0;
+  int n = 0;
+  bool ok = true;
+  for (int segs = 0; ok; ++segs) {
+    const int slot = segs % kSegs;
+    ok = wait(&bar->seg_full[slot], (segs / kSegs) & 1, 0x350);
+    if (!ok || !segments[slot].valid) break;
+    int lo, hi;
+    range(segments[slot], &lo, &hi);
+    mbar_arrive_warp(&bar->seg_empty[slot], lane);
+    if (lo >= hi) continue;
+    if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300) && wait_half(n, 0))) break;
+    issue_first(n, 0);
+    if (!(ok = wait_half(n, 1))) break;
+    issue_first(n, 1);
+    for (int i = lo; i < hi; ++i, ++n) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const uint64_t dr = dr0 + ((((2 * n + g) & 3) * kTile) >> 4);
+        if (i + 1 < hi && !(ok = ok && wait_half(n + 1, g))) break;      // (there long before its turn)
+        if (!(ok = ok && wait(&back_full[g], n & 1, 0x340 + which))) break;
+        if (g == 0 && i == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
+#pragma unroll
+        for (int q = 0; q < kHalf / 16; ++q)
+          umma_ts_elected(d_acc, d_first + g * kHalf + (q / 2) * kCols + (q % 2) * 8, dr + ((q * 2048) >> 4), idesc_acc,
+                          g > 0 || q > 0 || i > lo ? 1u : 0u, issuer);
+        umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
+        if (i + 1 < hi) issue_first(n + 1, g);
+      }
+      if (!ok) break;
+    }
+    if (!ok) break;
+    umma_commit_elected(&bar->keep_empty, issuer);
+    umma_commit_elected(&bar->acc_done, issuer);
+    ++keeps;
+  }
+}
+
 }  // namespace
 
 // ------------------------------------------------------------------ gradients of keys and values
-template <int D, bool BF16, bool GENERAL>
+template <int D, bool BF16, bool CAPPED, bool BIASED>
 __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid_constant__ BackwardParams p) {
   using LO = Layout<D>;
   constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile, kHalfTile = LO::kHalfTile;
@@ -360,66 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
   } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------ MMA: warp 0 S^T = K Q^T and dV += P^T dO, warp 1 dP^T = V dO^T and dK += dS^T Q
     const int which = warp - kMmaWarp;
-    const uint32_t issuer = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(BF16, kKeys, kHalf, false, false);
-    const uint32_t idesc_acc = umma_idesc_f16(BF16, kKeys, D, false, true);
-    const uint64_t da = umma_desc_sw128(smem_u32(smem + (which == 0 ? LO::kOffA : LO::kOffB)), 16, 1024);
-    // the first product's second operand (Q or dO) K-major, the second product's (dO or Q) with the rows as the reduction
-    const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kHalfTile), 16, 1024);
-    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + (which ^ 1) * kHalfTile), kHalf * 128, 1024);
-    const uint32_t d_first = tmem_base + (which == 0 ? kColS : kColDp), d_acc = tmem_base + kColAcc + which * D;
-    uint64_t* first_full = which == 0 ? bar->s_full : bar->dp_full;
-    uint64_t* back_full = which == 0 ? bar->p_full : bar->ds_full;
-    auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
-      const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
-      tc_fence_after_sync();
-      return r;
-    };
-    // the first product of half g of the rows of tile n: stage 2 n + g of the ring
-    auto issue_first = [&](int n, int g) {
-      const uint64_t db = db0 + ((((2 * n + g) & 3) * kTile) >> 4);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-        umma_ss_elected(d_first + g * kHalf, da + (((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4), db + (((i / 4) * (kHalf * 128) + (i % 4) * 32) >> 4),
-                        idesc_s, i > 0 ? 1u : 0u, issuer);
-      umma_commit_elected(&first_full[g], issuer);
-    };
-    auto wait_half = [&](int n, int g) { return wait(&bar->full[(2 * n + g) & 3], (n >> 1) & 1, 0x310 + g); };
-    uint32_t keeps = 0;
-    int n = 0;
-    bool ok = true;
-    for (int segs = 0; ok; ++segs) {
-      const int slot = segs % kSegs;
-      ok = wait(&bar->seg_full[slot], (segs / kSegs) & 1, 0x350);
-      if (!ok || !segments[slot].valid) break;
-      const int lo = segments[slot].lo, hi = segments[slot].hi;
-      mbar_arrive_warp(&bar->seg_empty[slot], lane);
-      if (lo >= hi) continue;
-      if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300) && wait_half(n, 0))) break;
-      issue_first(n, 0);
-      if (!(ok = wait_half(n, 1))) break;
-      issue_first(n, 1);
-      for (int i = lo; i < hi; ++i, ++n) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const uint64_t dr = dr0 + ((((2 * n + g) & 3) * kTile) >> 4);
-          if (i + 1 < hi && !(ok = ok && wait_half(n + 1, g))) break;      // (there long before its turn)
-          if (!(ok = ok && wait(&back_full[g], n & 1, 0x340 + which))) break;
-          if (g == 0 && i == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
-#pragma unroll
-          for (int q = 0; q < kHalf / 16; ++q)
-            umma_ts_elected(d_acc, d_first + g * kHalf + (q / 2) * kCols + (q % 2) * 8, dr + ((q * 2048) >> 4), idesc_acc,
-                            g > 0 || q > 0 || i > lo ? 1u : 0u, issuer);
-          umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
-          if (i + 1 < hi) issue_first(n + 1, g);
-        }
-        if (!ok) break;
-      }
-      if (!ok) break;
-      umma_commit_elected(&bar->keep_empty, issuer);
-      umma_commit_elected(&bar->acc_done, issuer);
-      ++keeps;
-    }
+    issue_products<D, BF16>(smem, bar, tmem_base, segments, which, lane, which ^ 1, [](const KeySegment& s, int* lo, int* hi) { *lo = s.lo, *hi = s.hi; });
   } else {
     // ------------------------------------------------------------ arithmetic: thread a key and a quarter of the tile's rows; warps 0-7 the
     // first half of them, 8-15 the second, each half with buffers of its own
@@ -470,8 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
           uint32_t sv[32];
           tmem_ld_x32_wait(s_col, sv);
           // (w holds what dS is the product of with dP - delta: first 1 - tanh^2, then that times the weight)
-          if constexpr (GENERAL) {
-            if (p.cap_out != 0.f) {
+          if constexpr (CAPPED) {
               capped(sv, p.cap_in, 1.0f);
               const uint64_t one2 = pack_f32x2(1.0f, 1.0f), out2 = pack_f32x2(p.cap_out, p.cap_out);
 #pragma unroll
@@ -482,9 +495,10 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
                 unpack_f32x2(mul_f32x2(t, out2), y0, y1);
                 sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
-            }
+          }
+          if constexpr (BIASED) {
             if (p.slopes != nullptr) {
-              const float sc = p.cap_out != 0.f ? 1.0f : p.score_log2, at = static_cast<float>(key);
+              const float sc = CAPPED ? 1.0f : p.score_log2, at = static_cast<float>(key);
               const uint64_t sc2 = pack_f32x2(sc, sc), at2 = pack_f32x2(-at, -at);
 #pragma unroll
               for (int u = 0; u < 32; u += 4) {
@@ -540,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
               pk[v] = pack2<BF16>(p0, p1);
               pk[v + 1] = pack2<BF16>(p2, p3);
               uint64_t w01 = p01, w23 = p23;
-              if (GENERAL && p.cap_out != 0.f) w01 = mul_f32x2(w01, pack_f32x2(w[u], w[u + 1])), w23 = mul_f32x2(w23, pack_f32x2(w[u + 2], w[u + 3]));
+              if constexpr (CAPPED) w01 = mul_f32x2(w01, pack_f32x2(w[u], w[u + 1])), w23 = mul_f32x2(w23, pack_f32x2(w[u + 2], w[u + 3]));
               if constexpr (!BF16) w01 = mul_f32x2(w01, pack_f32x2(f, f)), w23 = mul_f32x2(w23, pack_f32x2(f, f));
               unpack_f32x2(w01, w[u], w[u + 1]);
               unpack_f32x2(w23, w[u + 2], w[u + 3]);
@@ -675,7 +689,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_key_parts_kernel(const __grid
 }  // namespace
 
 // ------------------------------------------------------------------ gradients of queries
-template <int D, bool BF16, bool GENERAL>
+template <int D, bool BF16, bool CAPPED, bool BIASED>
 __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __grid_constant__ BackwardParams p) {
   using LO = Layout<D>;
   constexpr int kAtoms = LO::kAtoms, kTile = LO::kTile, kHalfTile = LO::kHalfTile;
@@ -695,11 +709,11 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&bar->s_full[g], 1);
-      mbar_init(&bar->s_taken[g], kComputeWarps / 2);
+      mbar_init(&bar->p_full[g], kComputeWarps / 2);
       mbar_init(&bar->dp_full[g], 1);
       mbar_init(&bar->ds_full[g], kComputeWarps / 2);
     }
-    mbar_init(&bar->acc_done, 1);
+    mbar_init(&bar->acc_done, 2);
     mbar_init(&bar->acc_free, kComputeWarps);
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&bar->seg_full[i], 1);
@@ -762,76 +776,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       }
     }
   } else if (warp >= kMmaWarp) {
-    // ------------------------------------------------------------ MMA: warp 0 S = Q K^T, warp 1 dP = dO V^T and dQ += dS K; a block of keys in halves
-    const int which = warp - kMmaWarp;
-    const uint32_t issuer = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kHalf, false, false);
-    const uint32_t idesc_acc = umma_idesc_f16(BF16, kRows, D, false, true);
-    const uint64_t da = umma_desc_sw128(smem_u32(smem + (which == 0 ? LO::kOffA : LO::kOffB)), 16, 1024);
-    const uint64_t db0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing + which * kHalfTile), 16, 1024);
-    const uint64_t dr0 = umma_desc_sw128(smem_u32(smem + LO::kOffRing), kHalf * 128, 1024);
-    const uint32_t d_first = tmem_base + (which == 0 ? kColS : kColDp);
-    uint64_t* first_full = which == 0 ? bar->s_full : bar->dp_full;
-    auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
-      const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
-      tc_fence_after_sync();
-      return r;
-    };
-    // S or dP of half g of block n: stage 2 n + g of the ring
-    auto issue_first = [&](int n, int g) {
-      const uint64_t db = db0 + ((((2 * n + g) & 3) * kTile) >> 4);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-        umma_ss_elected(d_first + g * kHalf, da + (((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4), db + (((i / 4) * (kHalf * 128) + (i % 4) * 32) >> 4),
-                        idesc_s, i > 0 ? 1u : 0u, issuer);
-      umma_commit_elected(&first_full[g], issuer);
-    };
-    auto wait_half = [&](int n, int g) { return wait(&bar->full[(2 * n + g) & 3], (n >> 1) & 1, 0x310 + g); };
-    uint32_t keeps = 0;
-    int n = 0;
-    bool ok = true;
-    for (int segs = 0; ok; ++segs) {
-      const int slot = segs % kSegs;
-      ok = wait(&bar->seg_full[slot], (segs / kSegs) & 1, 0x350);
-      if (!ok || !segments[slot].valid) break;
-      const int lo = segments[slot].lo0, hi = segments[slot].hi0;
-      mbar_arrive_warp(&bar->seg_empty[slot], lane);
-      if (lo >= hi) continue;
-      if (!(ok = wait(&bar->keep_full, keeps & 1, 0x300))) break;
-      if (which == 0) {
-        // scores go out as soon as the last ones have been read
-        for (int j = lo; ok && j < hi; ++j, ++n)
-          for (int g = 0; g < 2; ++g) {
-            if (!(ok = wait_half(n, g) && wait(&bar->s_taken[g], (n & 1) ^ 1, 0x330))) break;
-            issue_first(n, g);
-            umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
-          }
-      } else {
-        for (int g = 0; g < 2; ++g) {
-          if (!(ok = ok && wait_half(n, g))) break;
-          issue_first(n, g);
-        }
-        for (int j = lo; ok && j < hi; ++j, ++n)
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (j + 1 < hi && !(ok = ok && wait_half(n + 1, g))) break;
-            if (!(ok = ok && wait(&bar->ds_full[g], n & 1, 0x340))) break;
-            if (g == 0 && j == lo && !(ok = wait(&bar->acc_free, (keeps & 1) ^ 1, 0x320))) break;      // (at once the first time)
-            const uint64_t dr = dr0 + ((((2 * n + g) & 3) * kTile) >> 4);
-#pragma unroll
-            for (int q = 0; q < kHalf / 16; ++q)
-              umma_ts_elected(tmem_base + kColAcc, d_first + g * kHalf + (q / 2) * kCols + (q % 2) * 8, dr + ((q * 2048) >> 4), idesc_acc,
-                              g > 0 || q > 0 || j > lo ? 1u : 0u, issuer);
-            umma_commit_elected(&bar->empty[(2 * n + g) & 3], issuer);
-            if (j + 1 < hi) issue_first(n + 1, g);
-          }
-        if (!ok) break;
-        umma_commit_elected(&bar->acc_done, issuer);
-      }
-      if (!ok) break;
-      umma_commit_elected(&bar->keep_empty, issuer);
-      ++keeps;
-    }
+    // ------------------------------------------------------------ MMA: warp 0 S = Q K^T and P K, warp 1 dP = dO V^T and dS K
+    issue_products<D, BF16>(smem, bar, tmem_base, segments, warp - kMmaWarp, lane, 0, [](const Segment<1>& s, int* lo, int* hi) { *lo = s.lo0, *hi = s.hi0; });
   } else {
     // ------------------------------------------------------------ arithmetic: thread a row and a quarter of the block's keys
     const int quad = warp & 3, part_of_row = warp >> 2, g = warp >> 3, row = quad * 32 + lane;
@@ -839,7 +785,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
     const float c = p.c;
     float up, down;
     ds_scale<BF16>(p, &up, &down);
-    const float f = BF16 ? 1.0f : up * (1.0f / 16384.0f);
+    const float p_down = BF16 ? 1.0f : 1.0f / 16384.0f, f = BF16 ? 1.0f : up * p_down;
+    float* sums = reinterpret_cast<float*>(smem + LO::kOffRows);      // [2][4][128]: of dS, to set delta right
     const int r_half = row / kHalf, r_in = row % kHalf, r_token = r_half * p.half_tokens + r_in / p.half_heads,
               r_head = r_half * p.head_step + r_in % p.half_heads;
     const bool row_used = r_in < p.half_rows && r_head < p.group;
@@ -854,8 +801,8 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       if (!s.valid) break;
       const int lo = s.lo0, hi = s.hi0, token = s.first_token + r_token, pos = token + s.keys - s.tokens;
       const bool valid = row_used && token < s.tokens;
-      const HalfRows& rows = p.rows[((static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + s.first_token / p.tile_tokens) * 2 + r_half];
-      const float off = rows.lse[r_in], delta = rows.delta[r_in], slope = GENERAL ? rows.slope[r_in] : 0.f;
+      HalfRows& rows = p.rows[((static_cast<size_t>(s.seq) * p.kv_heads + s.kv_head) * p.tiles + s.first_token / p.tile_tokens) * 2 + r_half];
+      const float off = rows.lse[r_in], delta = rows.delta[r_in], slope = BIASED ? rows.slope[r_in] : 0.f;
       int limit = valid ? visible_keys(pos, s.keys, p.causal, s.prefix) : 0, low = 0, doc = -1;
       bool mixed = false;
       if (p.documents != nullptr) {
@@ -868,6 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         }
         mixed = p.mixed[s.seq] != 0;
       }
+      uint64_t sum2 = 0;
       const int limit_of_all = __reduce_min_sync(0xffffffffu, limit), low_of_all = __reduce_max_sync(0xffffffffu, low);
       const bool behind = p.causal && s.prefix <= s.keys - s.tokens + s.first_token + 1;      // every key that a row sees is at or in front of it
       for (int j = lo; j < hi; ++j, ++n) {
@@ -877,11 +825,11 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         const int k0 = j * kKeys + part_of_row * kCols;
         const bool cut = limit_of_all < k0 + kCols, cut_low = low_of_all > k0;
         float w[kCols] = {};
+        [[maybe_unused]] float weight[CAPPED ? kCols : 1];      // without the cap's factor
         {
           uint32_t sv[32];
           tmem_ld_x32_wait(lane_base + kColS + part_of_row * kCols, sv);
-          if constexpr (GENERAL) {
-            if (p.cap_out != 0.f) {
+          if constexpr (CAPPED) {
               capped(sv, p.cap_in, 1.0f);
               const uint64_t one2 = pack_f32x2(1.0f, 1.0f), out2 = pack_f32x2(p.cap_out, p.cap_out);
 #pragma unroll
@@ -892,8 +840,9 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
                 unpack_f32x2(mul_f32x2(t, out2), y0, y1);
                 sv[u] = __float_as_uint(y0), sv[u + 1] = __float_as_uint(y1);
               }
-            }
-            if (p.slopes != nullptr) biased(sv, p.cap_out != 0.f ? 1.0f : p.score_log2, -slope, static_cast<float>(pos - k0), behind);
+          }
+          if constexpr (BIASED) {
+            if (p.slopes != nullptr) biased(sv, CAPPED ? 1.0f : p.score_log2, -slope, static_cast<float>(pos - k0), behind);
           }
           if (mixed) {
             const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
@@ -915,32 +864,46 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
               if (u >= lim) sv[u] = __float_as_uint(-INFINITY);
           }
           const uint64_t c2 = pack_f32x2(c, c), off2 = pack_f32x2(off, off);
+          uint32_t pk[16];
 #pragma unroll
           for (int u = 0; u < 32; u += 2) {
             uint64_t x = softmax_weights(sv[u], sv[u + 1], c2, off2, false);
-            if (GENERAL && p.cap_out != 0.f) x = mul_f32x2(x, pack_f32x2(w[u], w[u + 1]));
+            if constexpr (CAPPED) {
+              unpack_f32x2(x, weight[u], weight[u + 1]);
+              x = mul_f32x2(x, pack_f32x2(w[u], w[u + 1]));
+            }
+            float p0, p1;
+            unpack_f32x2(x, p0, p1);
+            pk[u / 2] = pack2<BF16>(p0, p1);
             if constexpr (!BF16) x = mul_f32x2(x, pack_f32x2(f, f));
             unpack_f32x2(x, w[u], w[u + 1]);
           }
+          tmem_st_x16(lane_base + kColS + part_of_row * kCols, pk);
         }
+        tmem_wait_st();
         tc_fence_before_sync();
-        mbar_arrive_warp(&bar->s_taken[g], lane);
+        mbar_arrive_warp(&bar->p_full[g], lane);
 
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->dp_full[g], n & 1, abort_word, 0x810));
         if (!ok) break;
         tc_fence_after_sync();
         const uint32_t dp_col = lane_base + kColDp + part_of_row * kCols;
-        {
-          const uint64_t delta2 = pack_f32x2(delta, delta);
-          uint32_t dp[32], pk[16];
-          tmem_ld_x32_wait(dp_col, dp);
+        const uint64_t delta2 = pack_f32x2(delta, delta);
 #pragma unroll
-          for (int u = 0; u < 32; u += 2) {
+        for (int c0 = 0; c0 < kCols; c0 += 16) {
+          uint32_t dp[16], pk[8];
+          tmem_ld_x16_wait(dp_col + c0, dp);
+#pragma unroll
+          for (int u = 0; u < 16; u += 2) {
+            const uint64_t d = add_f32x2(pack_f32x2(__uint_as_float(dp[u]), __uint_as_float(dp[u + 1])), delta2),
+                           x = mul_f32x2(pack_f32x2(w[c0 + u], w[c0 + u + 1]), d);
+            if constexpr (CAPPED) sum2 = fma_f32x2(pack_f32x2(weight[c0 + u], weight[c0 + u + 1]), d, sum2);
+            else sum2 = add_f32x2(sum2, x);
             float x0, x1;
-            unpack_f32x2(mul_f32x2(pack_f32x2(w[u], w[u + 1]), add_f32x2(pack_f32x2(__uint_as_float(dp[u]), __uint_as_float(dp[u + 1])), delta2)), x0, x1);
+            unpack_f32x2(x, x0, x1);
             pk[u / 2] = pack2<BF16>(x0, x1);
           }
-          tmem_st_x16(dp_col, pk);
+          tmem_st_x8(dp_col + c0 / 2, pk);
         }
         tmem_wait_st();
         tc_fence_before_sync();
@@ -955,17 +918,31 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         if (!ok) break;
         tc_fence_after_sync();
       }
-      const float scale = p.scale * down;
+      // What delta is off by: the sum of the row's P (dP - delta), which is 0 for the right one.  delta comes from a result that is rounded, and
+      // was summed from rounded weights: a step of the type relative to a difference that can be small beside it where few keys have the weight.
+      // dS misses -P times that (and the cap's factor), so dQ misses it times P K; the keys' kernel, behind this one, gets delta set right.
+      float s0, s1;
+      unpack_f32x2(sum2, s0, s1);
+      float* mine = sums + (segs & 1) * 512 + row;
+      mine[part_of_row * 128] = s0 + s1;
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      const float off_by = (mine[0] + mine[128] + mine[256] + mine[384]) * (CAPPED ? p_down : down);
+      if (part_of_row == 0 && valid) rows.delta[r_in] = delta - off_by;
+      const float scale = p.scale * down, scale_pk = -p.scale * off_by * p_down;
       uint8_t* dst = static_cast<uint8_t*>(p.dq) + 2 * ((static_cast<size_t>(s.seq) * p.M + token) * p.heads + s.kv_head * p.group + r_head) * p.d;
 #pragma unroll
       for (int cc = 0; cc < D / 4; cc += 16) {
         const int col = part_of_row * (D / 4) + cc;
-        uint32_t x[16];
+        float x[16];
         if (has) {
-          tmem_ld_x16_wait(lane_base + kColAcc + col, x);
+          uint32_t ds[16], pk[16];
+          tmem_ld_x16_wait(lane_base + kColAcc + D + col, ds);
+          tmem_ld_x16_wait(lane_base + kColAcc + col, pk);
+#pragma unroll
+          for (int u = 0; u < 16; ++u) x[u] = fmaf(__uint_as_float(pk[u]), scale_pk, __uint_as_float(ds[u]) * scale);
         } else {
 #pragma unroll
-          for (int u = 0; u < 16; ++u) x[u] = 0u;
+          for (int u = 0; u < 16; ++u) x[u] = 0.f;
         }
         if (cc + 16 == D / 4) {
           tc_fence_before_sync();
@@ -976,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
         for (int u = 0; u < 16; u += 8) {
           uint32_t v[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] = pack2<BF16>(__uint_as_float(x[u + 2 * q]) * scale, __uint_as_float(x[u + 2 * q + 1]) * scale);
+          for (int q = 0; q < 4; ++q) v[q] = pack2<BF16>(x[u + 2 * q], x[u + 2 * q + 1]);
           if (col + u < p.d) *reinterpret_cast<uint4*>(dst + 2 * (col + u)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
@@ -1010,10 +987,10 @@ cudaLaunchConfig_t config(long long grid, int threads, int smem, cudaStream_t st
   return cfg;
 }
 
-template <int D, bool BF16, bool GENERAL>
+template <int D, bool BF16, bool CAPPED, bool BIASED>
 cudaError_t launch_products(const BackwardParams& p, int sms, cudaStream_t stream) {
-  auto keys = backward_keys_kernel<D, BF16, GENERAL>;
-  auto queries = backward_queries_kernel<D, BF16, GENERAL>;
+  auto keys = backward_keys_kernel<D, BF16, CAPPED, BIASED>;
+  auto queries = backward_queries_kernel<D, BF16, CAPPED, BIASED>;
   static std::atomic<unsigned long long> configured{0};
   int dev = 0;
   cudaError_t e = current_device_checked(&dev);
@@ -1025,9 +1002,9 @@ cudaError_t launch_products(const BackwardParams& p, int sms, cudaStream_t strea
     mark_device_configured(configured, dev);
   }
   cudaLaunchAttribute attr[1];
-  e = launch_kernel(config(sms, kThreads, Layout<D>::kBytes, stream, attr), keys, p);
+  e = launch_kernel(config(p.items < sms ? p.items : sms, kThreads, Layout<D>::kBytes, stream, attr), queries, p);      // (sets delta right)
+  if (e == cudaSuccess) e = launch_kernel(config(sms, kThreads, Layout<D>::kBytes, stream, attr), keys, p);
   if (e == cudaSuccess) e = launch_kernel(config(sms, kSumThreads, 0, stream, attr, kSumSlices), sum_key_parts_kernel<D, BF16>, p);
-  if (e == cudaSuccess) e = launch_kernel(config(p.items < sms ? p.items : sms, kThreads, Layout<D>::kBytes, stream, attr), queries, p);
   return e;
 }
 
@@ -1043,8 +1020,8 @@ cudaError_t launch_backward(const BackwardParams& p, int sms, cudaStream_t strea
   const cudaLaunchConfig_t rows = config(2 * p.items < 8 * sms ? 2 * p.items : 8 * sms, kRowThreads, 0, stream, attr);
   const cudaError_t e = D == 64 ? launch_kernel(rows, backward_rows_kernel<BF16, 8>, p) : launch_kernel(rows, backward_rows_kernel<BF16, 16>, p);
   if (e != cudaSuccess) return e;
-  const bool general = p.cap_out != 0.f || p.slopes != nullptr;
-  return general ? launch_products<D, BF16, true>(p, sms, stream) : launch_products<D, BF16, false>(p, sms, stream);
+  if (p.cap_out != 0.f) return launch_products<D, BF16, true, true>(p, sms, stream);      // (with slopes or without)
+  return p.slopes != nullptr ? launch_products<D, BF16, false, true>(p, sms, stream) : launch_products<D, BF16, false, false>(p, sms, stream);
 }
 
 template cudaError_t launch_backward<(DITTO_MASKED_BACKWARD_PART & 1) ? 128 : 64, (DITTO_MASKED_BACKWARD_PART & 2) != 0>(const BackwardParams&, int,
