@@ -62,6 +62,15 @@ int set_rules(masked::Params& p, float scale, float cap, const float* slopes, co
   return DITTO_OK;
 }
 
+// The forward kernel's units for a bias without a cap.  Its product brings the bias in units of the raw scores, slope / scale: scales so far out
+// that this could leave the range of fp32 keep the bias in units of the exponent.
+void set_bias_units(masked::Params& p, float scale) {
+  p.bias_unit = kLog2e, p.bias_factor = p.score_log2, p.bias_product = 0;
+  if (p.slopes == nullptr || p.cap_out != 0.f || scale < 0x1p-20f || scale > 0x1p20f) return;
+  p.bias_unit = 1.0f / scale, p.bias_factor = 1.0f, p.bias_product = 1;
+  p.c = p.score_log2;
+}
+
 int check_heads(int heads, int kv_heads, int d, int dtype) {
   if (heads <= 0 || kv_heads <= 0 || d <= 0) return DITTO_ERR_INVALID_ARG;
   if (dtype != DITTO_DTYPE_FP16 && dtype != DITTO_DTYPE_BF16) return DITTO_ERR_UNSUPPORTED;
@@ -236,6 +245,7 @@ int ditto_b200_masked_attention(const ditto_b200_masked_args* a, void* workspace
   masked::Params p;
   rc = fill_masked(p, a);
   if (rc) return rc;
+  set_bias_units(p, a->scale);
   const MaskedScratch ws = masked_scratch(a, false, 0);
   if (ws.bytes > 0 && (workspace == nullptr || ws_bytes < ws.bytes)) return DITTO_ERR_WORKSPACE;
   if (ws.bytes > 0 && !aligned16(workspace)) return DITTO_ERR_INVALID_ARG;
@@ -350,6 +360,7 @@ int ditto_b200_paged_attention(const ditto_b200_paged_args* a, void* workspace, 
   std::memset(&p, 0, sizeof(p));
   rc = set_rules(p, a->scale, a->cap, a->slopes, a->prefix, 1);
   if (rc) return rc;
+  set_bias_units(p, a->scale);
   PagedPlan plan;
   rc = paged_plan(a, &plan);
   if (rc) return rc;

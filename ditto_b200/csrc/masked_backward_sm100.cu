@@ -172,7 +172,7 @@ struct Layout {
 struct Bars {
   uint64_t keep_full, keep_empty;
   uint64_t full[4], empty[4];
-  uint64_t s_full[2], p_full[2], dp_full[2], ds_full[2], acc_done, acc_free;
+  uint64_t s_full[2], p_full[2], dp_full[2], ds_full[2], acc_done, acc_free, sums_full;
   uint64_t seg_full[kSegs], seg_empty[kSegs];
   uint32_t tmem_base, abort_word;
   int start_item, start_tile, left, per_cta;
@@ -715,6 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
     }
     mbar_init(&bar->acc_done, 2);
     mbar_init(&bar->acc_free, kComputeWarps);
+    mbar_init(&bar->sums_full, kComputeWarps);
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&bar->seg_full[i], 1);
       mbar_init(&bar->seg_empty[i], kComputeWarps + 2);
@@ -925,7 +926,9 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       unpack_f32x2(sum2, s0, s1);
       float* mine = sums + (segs & 1) * 512 + row;
       mine[part_of_row * 128] = s0 + s1;
-      asm volatile("bar.sync 1, 512;" ::: "memory");
+      mbar_arrive_warp(&bar->sums_full, lane);
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar->sums_full, segs & 1, abort_word, 0x850));
+      if (!ok) break;
       const float off_by = (mine[0] + mine[128] + mine[256] + mine[384]) * (CAPPED ? p_down : down);
       if (part_of_row == 0 && valid) rows.delta[r_in] = delta - off_by;
       const float scale = p.scale * down, scale_pk = -p.scale * off_by * p_down;

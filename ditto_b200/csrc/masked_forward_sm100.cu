@@ -42,7 +42,8 @@ struct Layout {
   static constexpr int kTile = 128 * D * 2;
   static constexpr int kStages = D == 128 ? (NT == 2 ? 4 : 5) : 8;     // K and V blocks in turn
   static constexpr int kOffKV = NT * kTile;
-  static constexpr int kOffSum = kOffKV + kStages * kTile;             // [2][buffer][128] references and sums
+  static constexpr int kOffBias = kOffKV + kStages * kTile;            // what the product of the bias reads
+  static constexpr int kOffSum = kOffBias + kRows * 128;               // [2][buffer][128] references and sums
   static constexpr int kOffBar = kOffSum + 4096;
   static constexpr int kOffSeg = kOffBar + 1024;
   static constexpr int kBytes = kOffSeg + 512 + 1024;
@@ -53,12 +54,32 @@ struct Bars {
   uint64_t kv_full[8], kv_empty[8];
   uint64_t s_full[2], p_part[2][2], o_done[2], o_free[2];
   uint64_t seg_full[kSegs], seg_empty[kSegs];
-  uint64_t turn[2];
+  uint64_t turn[2], sums_full;
   uint32_t tmem_base, abort_word;
   PagedStart start;
   int scan[kThreads / 32 + 1];
 };
 static_assert(sizeof(Bars) <= 1024, "barrier block too large");
+
+// The bias by distance as a 16-wide step more of the scores' product, for rows that see no key behind them: -slope (pos - k0 - i) is
+// slope i, which the step adds, plus a number per row and block, slope (k0 - pos), which goes into the row's maximum and the exponents' offset.
+// The step's rows hold the slope (over the scale) as a sum of three bf16, 24 bits; its columns the key's place i in the block three times, which
+// bf16 holds exactly.  One buffer of 128 rows of 128 bytes, swizzled like the tiles: the slopes of tile 0 in bytes 0 to 31 of a row, those of tile 1 in
+// 32 to 63, the places in 64 to 95.
+__device__ __forceinline__ uint8_t* bias_at(uint8_t* buffer, int row, int sixteenths) { return buffer + row * 128 + ((sixteenths ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint2 bias_terms(float x) {
+  const __nv_bfloat16 a = __float2bfloat16(x);
+  x -= __bfloat162float(a);
+  const __nv_bfloat16 b = __float2bfloat16(x);
+  x -= __bfloat162float(b);
+  const __nv_bfloat16 c = __float2bfloat16(x);
+  return make_uint2(__bfloat16_as_ushort(a) | static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16, __bfloat16_as_ushort(c));
+}
+// Whether every key that a row of tile t sees is at or in front of it.
+template <int NT>
+__device__ __forceinline__ bool keys_in_front(const Params& p, const Segment<NT>& s, int t) {
+  return p.causal && s.prefix <= s.keys - s.tokens + s.first_token + t * p.tile_tokens + 1;
+}
 
 // Shares of a paged call: the blocks of all items, in order, in gridDim.x equal shares.
 template <int NT>
@@ -124,7 +145,7 @@ __device__ __forceinline__ void find_start(const Params& p, Bars* bar) {
 
 }  // namespace
 
-template <int D, bool BF16, int NT, bool PAGED>
+template <int D, bool BF16, int NT, bool PAGED, bool CAPPED, bool BIASED>
 __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __grid_constant__ Params p) {
   using LO = Layout<D, NT>;
   constexpr int kStages = LO::kStages, kAtoms = LO::kAtoms, kTile = LO::kTile;
@@ -145,6 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       mbar_init(&bar->turn[i], 1);
       mbar_init(&bar->o_free[i], NT == 2 ? kSoftmaxWarps / 2 : kSoftmaxWarps);
     }
+    mbar_init(&bar->sums_full, kSoftmaxWarps);
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&bar->seg_full[i], 1);
       mbar_init(&bar->seg_empty[i], kSoftmaxWarps + 2);
@@ -159,6 +181,16 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
   if (warp == 0) {
     tmem_alloc(&bar->tmem_base, kTmemCols);
     tmem_relinquish();
+  }
+  constexpr bool kBiasProduct = BIASED && !CAPPED;
+  if constexpr (kBiasProduct) {
+    uint8_t* bias = smem + LO::kOffBias;
+    for (int i = threadIdx.x; i < kRows * 8; i += kThreads) {
+      const int row = i >> 3, piece = i & 7;
+      const uint32_t place = __bfloat16_as_ushort(__int2bfloat16_rn(row));
+      *reinterpret_cast<uint4*>(bias_at(bias, row, piece)) = piece == 4 ? make_uint4(place | place << 16, place, 0, 0) : make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
   }
   if (warp == kProducerWarp && lane == 0) {
     tma_prefetch_desc(&p.map_q);
@@ -214,6 +246,15 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->q_empty[t], ((loads_q >> t) & 1) ^ 1, abort_word, 0x100 + t));
         if (!ok) break;
         loads_q ^= 1u << t;
+        if constexpr (kBiasProduct) {
+          const bool brought = p.bias_product && keys_in_front(p, s, t);
+          for (int row = lane; row < kRows; row += 32) {
+            const float slope = brought ? p.slopes[s.kv_head * p.group + row % p.group] * p.bias_unit : 0.f;
+            *reinterpret_cast<uint2*>(bias_at(smem + LO::kOffBias, row, 2 * t)) = bias_terms(slope);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         if (lane == 0) {
           mbar_arrive_expect_tx(&bar->q_full[t], q_bytes);
           for (int a = 0; a < kAtoms; ++a)
@@ -269,6 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     const uint64_t dq = umma_desc_sw128(smem_u32(smem + t * kTile), 16, 1024);
     const uint64_t dk0 = umma_desc_sw128(smem_u32(smem + LO::kOffKV), 16, 1024);
     const uint64_t dv0 = umma_desc_sw128(smem_u32(smem + LO::kOffKV), kKeys * 128, 1024);
+    [[maybe_unused]] const uint32_t idesc_bias = umma_idesc_f16(true, kRows, kKeys, false, false);
+    [[maybe_unused]] const uint64_t dbias = umma_desc_sw128(smem_u32(smem + LO::kOffBias), 16, 1024);
     const uint32_t d_o = tmem_base + kColO + buf * D, d_s = tmem_base + buf * kKeys;
     auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
       const bool r = __all_sync(0xffffffffu, mbar_wait(b, parity, abort_word, code));
@@ -290,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
         umma_ss_elected(d_s, dq + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
       }
+      if constexpr (kBiasProduct) umma_ss_elected(d_s, dbias + 2 * t, dbias + 4, idesc_bias, 1u, issuer);
       umma_commit_elected(&bar->s_full[buf], issuer);
       umma_commit_elected(&bar->kv_empty[st], issuer);
     };
@@ -423,12 +467,10 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           mixed = p.mixed[s.seq] != 0;
         }
       }
-      const float slope = p.slopes != nullptr && valid ? p.slopes[head] * 1.4426950408889634f : 0.f;
+      const float slope = BIASED && p.slopes != nullptr && valid ? p.slopes[head] * (CAPPED ? 1.4426950408889634f : p.bias_unit) : 0.f;
       // the first block that a row of this warp does not see whole, and the last one in which one does not see the first key (documents)
       const int cut = __reduce_min_sync(0xffffffffu, limit) / kKeys, cut_low = __reduce_max_sync(0xffffffffu, low);
-      const bool modified = p.cap_out != 0.f || p.slopes != nullptr || mixed;
-      // every key that a row sees is at or in front of it
-      const bool behind = p.causal && s.prefix <= s.keys - s.tokens + s.first_token + t * p.tile_tokens + 1;
+      const bool in_front = keys_in_front(p, s, t), brought = kBiasProduct && p.bias_product && in_front;
       RowReference ref(c);
       if (limit == 0) ref.m = 0.f, ref.large = false;      // sees nothing: asks for no rescale
       float l = 0.f;
@@ -440,17 +482,21 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         uint32_t sv[kKeys];
         tmem_ld_x128_wait(s_col, sv);
         const int k0 = j * kKeys;
-        if (modified) {
-          if (p.cap_out != 0.f) capped(sv, p.cap_in, p.cap_out);
-          if (p.slopes != nullptr) biased(sv, p.cap_out != 0.f ? 1.0f : p.score_log2, slope, static_cast<float>(pos - k0), behind);
-          if constexpr (!PAGED) {
-            if (mixed) {
-              const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
+        float base = 0.f;                              // what the row's scores in sv lack
+        if (CAPPED && p.cap_out != 0.f) {
+          capped(sv, p.cap_in, p.cap_out);
+          if (p.slopes != nullptr) biased(sv, 1.0f, slope, static_cast<float>(pos - k0), in_front);
+        } else if (BIASED) {
+          if (brought) base = slope * static_cast<float>(k0 - pos);
+          else biased(sv, p.bias_factor, slope, static_cast<float>(pos - k0), in_front);
+        }
+        if constexpr (!PAGED) {
+          if (mixed) {
+            const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
 #pragma unroll
-              for (int i = 0; i < kKeys; ++i) {
-                if (ids[min(k0 + i, p.L - 1)] != doc) sv[i] = __float_as_uint(-INFINITY);
-                if (i % 8 == 7) asm volatile("" ::: "memory");       // (eight ids at a time: registers)
-              }
+            for (int i = 0; i < kKeys; ++i) {
+              if (ids[min(k0 + i, p.L - 1)] != doc) sv[i] = __float_as_uint(-INFINITY);
+              if (i % 8 == 7) asm volatile("" ::: "memory");       // (eight ids at a time: registers)
             }
           }
         }
@@ -476,7 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
             else mx[u] = fmaxf(mx[u], __uint_as_float(sv[i + u]));
           }
         }
-        const float m_new = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], ref.m));
+        const float m_new = kBiasProduct ? fmaxf(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) + base, ref.m)
+                                         : max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], ref.m));
         const bool need = ref.asks(m_new, c, kRescaleThreshold) && m_new != -INFINITY;
         if (__any_sync(0xffffffffu, need)) {
           const float f = ref.move(m_new, c);
@@ -492,6 +539,11 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
             tmem_wait_st();
           }
           l *= f;
+          if (kBiasProduct && __any_sync(0xffffffffu, ref.large && base != 0.f)) {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) + base);
+            base = 0.f;
+          }
           ref.subtract(sv);
         }
         if constexpr (PAGED) {
@@ -507,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
             fence_proxy_async_smem();
           }
         }
-        const float mc = ref.offset(c);
+        const float mc = kBiasProduct ? fmaf(-base, c, ref.offset(c)) : ref.offset(c);
         const uint64_t c2 = pack_f32x2(c, c), nmc2 = pack_f32x2(-mc, -mc);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -548,7 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       if constexpr (NT == 1) {
         float2* both = sums + (segs & 1) * 256;
         both[buf * 128] = make_float2(ref.m, l);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        mbar_arrive_warp(&bar->sums_full, lane);
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->sums_full, segs & 1, abort_word, 0x850));
+        if (!ok) break;
         const float2 other = both[(buf ^ 1) * 128];
         const float m = other.y == 0.f ? ref.m : l == 0.f ? other.x : fmaxf(ref.m, other.x);
         f_mine = ref.m == m ? 1.0f : l == 0.f ? 0.f : ex2_approx((ref.m - m) * c);
@@ -639,9 +693,9 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
 
 namespace {
 
-template <int D, bool BF16, int NT, bool PAGED>
+template <int D, bool BF16, int NT, bool PAGED, bool CAPPED, bool BIASED>
 cudaError_t launch_one(const Params& p, int grid, cudaStream_t stream) {
-  auto kern = masked_forward_kernel<D, BF16, NT, PAGED>;
+  auto kern = masked_forward_kernel<D, BF16, NT, PAGED, CAPPED, BIASED>;
   static std::atomic<unsigned long long> configured{0};
   int dev = 0;
   cudaError_t e = current_device_checked(&dev);
@@ -666,9 +720,17 @@ cudaError_t launch_one(const Params& p, int grid, cudaStream_t stream) {
 
 }  // namespace
 
+namespace {
+template <int D, bool BF16, bool PAGED, bool CAPPED, bool BIASED>
+cudaError_t launch_tiles(const Params& p, int tiles, int grid, cudaStream_t stream) {
+  return tiles == 2 ? launch_one<D, BF16, 2, PAGED, CAPPED, BIASED>(p, grid, stream) : launch_one<D, BF16, 1, PAGED, CAPPED, BIASED>(p, grid, stream);
+}
+}  // namespace
+
 template <int D, bool BF16, bool PAGED>
 cudaError_t launch_forward(const Params& p, int tiles, int grid, cudaStream_t stream) {
-  return tiles == 2 ? launch_one<D, BF16, 2, PAGED>(p, grid, stream) : launch_one<D, BF16, 1, PAGED>(p, grid, stream);
+  if (p.cap_out != 0.f) return launch_tiles<D, BF16, PAGED, true, true>(p, tiles, grid, stream);      // (with slopes or without)
+  return p.slopes != nullptr ? launch_tiles<D, BF16, PAGED, false, true>(p, tiles, grid, stream) : launch_tiles<D, BF16, PAGED, false, false>(p, tiles, grid, stream);
 }
 
 template cudaError_t launch_forward<(DITTO_MASKED_PART & 1) ? 128 : 64, (DITTO_MASKED_PART & 2) != 0, (DITTO_MASKED_PART & 4) != 0>(

@@ -41,6 +41,10 @@ struct Params {
   float c;                    // factor of a score in the exponent of 2: scale log2(e), or 1 where cap or bias have applied it
   float cap_in, cap_out;      // scale / cap, and cap log2(e); cap_out 0: no cap
   float score_log2;           // scale log2(e)
+  // forward, slopes without a cap: a slope times bias_unit is in the units of the scores times bias_factor.  bias_product: the scores' product
+  // brings the bias of rows whose keys are all at or in front of them.
+  float bias_unit, bias_factor;
+  int bias_product;
   const float* slopes;        // [heads] or null
   const int* prefix;          // [batch] or null
   const int* documents;       // [batch, L] or null
@@ -248,8 +252,20 @@ __device__ __forceinline__ void capped(uint32_t (&s)[N], float k, float f) {
     s[i] = __float_as_uint(x0), s[i + 1] = __float_as_uint(x1);
     most = max3(most, fabsf(x0), fabsf(x1));
   }
-  if (__all_sync(0xffffffffu, most <= 0.75f)) {
-    auto both = [&](float c) { return pack_f32x2(f * c, f * c); };
+  auto both = [&](float c) { return pack_f32x2(f * c, f * c); };
+  if (__all_sync(0xffffffffu, most <= 0.35f)) {
+    const uint64_t c0 = both(1.0f), c1 = both(-0x1.555394p-2f), c2 = both(0x1.106164p-3f), c3 = both(-0x1.929fdep-5f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t x = pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), z = mul_f32x2(x, x);
+      uint64_t q = fma_f32x2(c3, z, c2);
+      q = fma_f32x2(q, z, c1);
+      q = fma_f32x2(q, z, c0);
+      float y0, y1;
+      unpack_f32x2(mul_f32x2(x, q), y0, y1);
+      s[i] = __float_as_uint(y0), s[i + 1] = __float_as_uint(y1);
+    }
+  } else if (__all_sync(0xffffffffu, most <= 0.75f)) {
     const uint64_t c0 = both(1.0f), c1 = both(-0x1.5554a4p-2f), c2 = both(0x1.10ed66p-3f), c3 = both(-0x1.b5604ep-5f), c4 = both(0x1.423392p-6f),
                    c5 = both(-0x1.389a58p-8f);
 #pragma unroll
@@ -271,17 +287,25 @@ __device__ __forceinline__ void capped(uint32_t (&s)[N], float k, float f) {
 }
 
 // s <- f s - slope |far - i| for scores of keys i = 0 .. N - 1 of a query `far` positions behind the first of them.  Where no key that the row
-// sees lies behind it (`linear`) the bias is linear in i: two instructions of the multiply-add pipe for two scores.
+// sees lies behind it (`linear`) the bias is linear in i: two instructions of the multiply-add pipe for two scores, with eight multiples of the
+// slope in registers (a multiple a score would have to be loaded as a constant, two instructions more).
 template <int N>
 __device__ __forceinline__ void biased(uint32_t (&s)[N], float f, float slope, float far, bool linear) {
   if (linear) {
-    const uint64_t f2 = pack_f32x2(f, f), slope2 = pack_f32x2(slope, slope), base2 = pack_f32x2(-slope * far, -slope * far);
+    const uint64_t f2 = pack_f32x2(f, f);
+    uint64_t near[4];
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint64_t bias = fma_f32x2(slope2, pack_f32x2(static_cast<float>(i), static_cast<float>(i + 1)), base2);
-      float y0, y1;
-      unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, bias), y0, y1);
-      s[i] = __float_as_uint(y0), s[i + 1] = __float_as_uint(y1);
+    for (int u = 0; u < 4; ++u) near[u] = pack_f32x2(slope * static_cast<float>(2 * u), slope * static_cast<float>(2 * u + 1));
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+      const float base = slope * (static_cast<float>(i) - far);
+      const uint64_t base2 = pack_f32x2(base, base);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float y0, y1;
+        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i + 2 * u]), __uint_as_float(s[i + 2 * u + 1])), f2, add_f32x2(near[u], base2)), y0, y1);
+        s[i + 2 * u] = __float_as_uint(y0), s[i + 2 * u + 1] = __float_as_uint(y1);
+      }
     }
   } else {
 #pragma unroll
