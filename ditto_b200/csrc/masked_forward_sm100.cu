@@ -36,15 +36,20 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kSegs = 4;                      // items that the producer is ahead of the others
 constexpr int kSplit = 96;                    // keys in the first part of P: their P V runs under the last exponentials
 
-template <int D, int NT>
+// SPLIT: items of a single token, whose heads (32 at most) fill a part of a tile only.  Four copies of the rows, at rows 0, 32, 64 and 96: a warp has
+// a quarter of a block's keys of each row instead of a thread a whole row, and no weight on the others; the copies' results are summed at an item's
+// end.  A block takes a quarter of the time, below that of its loads.  64 ragged sequences of up to 16384 keys, 32 heads over 8 of 128: 414 -> 363 us
+// (6.0 TB/s), of 64, 128 sequences: 730 -> 425 us (5.8 TB/s).
+template <int D, int NT, bool SPLIT>
 struct Layout {
   static constexpr int kAtoms = D / 64;
   static constexpr int kTile = 128 * D * 2;
-  static constexpr int kStages = D == 128 ? (NT == 2 ? 4 : 5) : 8;     // K and V blocks in turn
+  static constexpr int kStages = D == 128 ? (NT == 2 || SPLIT ? 4 : 5) : 8;     // K and V blocks in turn
   static constexpr int kOffKV = NT * kTile;
   static constexpr int kOffBias = kOffKV + kStages * kTile;            // what the product of the bias reads
   static constexpr int kOffSum = kOffBias + kRows * 128;               // [2][buffer][128] references and sums
-  static constexpr int kOffBar = kOffSum + 4096;
+  static constexpr int kOffJoin = kOffSum + 4096;                      // (SPLIT) [2][warp][32 rows][16] of the accumulators
+  static constexpr int kOffBar = kOffJoin + (SPLIT ? 2 * kSoftmaxWarps * 2048 : 0);
   static constexpr int kOffSeg = kOffBar + 1024;
   static constexpr int kBytes = kOffSeg + 512 + 1024;
 };
@@ -54,7 +59,7 @@ struct Bars {
   uint64_t kv_full[8], kv_empty[8];
   uint64_t s_full[2], p_part[2][2], o_done[2], o_free[2];
   uint64_t seg_full[kSegs], seg_empty[kSegs];
-  uint64_t turn[2], sums_full;
+  uint64_t turn[2], sums_full, join_full;
   uint32_t tmem_base, abort_word;
   PagedStart start;
   int scan[kThreads / 32 + 1];
@@ -81,16 +86,17 @@ __device__ __forceinline__ bool keys_in_front(const Params& p, const Segment<NT>
   return p.causal && s.prefix <= s.keys - s.tokens + s.first_token + t * p.tile_tokens + 1;
 }
 
-// Shares of a paged call: the blocks of all items, in order, in gridDim.x equal shares.
+// Shares of a paged call: the blocks of all items of a lane of heads, in order, in gridDim.x / lanes equal shares.
 template <int NT>
 __device__ __forceinline__ void find_start(const Params& p, Bars* bar) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int kWarps = kThreads / 32;
+  const int heads = p.kv_heads / p.lanes;
   int mine = 0, first_cost = 0;
   for (int b = tid; b < p.batch; b += kThreads) {
     Sequence q;
     q.load(p, b);
-    const int cost = p.kv_heads * q.template units_of_head<NT>(p);
+    const int cost = heads * q.template units_of_head<NT>(p);
     if (b == tid) first_cost = cost;
     mine += cost;
   }
@@ -101,8 +107,8 @@ __device__ __forceinline__ void find_start(const Params& p, Bars* bar) {
   __syncthreads();
   int total = 0;
   for (int w = 0; w < kWarps; ++w) total += bar->scan[w];
-  const int grid = gridDim.x, per = max(1, (total + grid - 1) / grid);
-  const int u0 = min(static_cast<long long>(per) * blockIdx.x, static_cast<long long>(total)), left = min(per, total - u0);
+  const int shares = gridDim.x / p.lanes, per = max(1, (total + shares - 1) / shares);
+  const int u0 = min(static_cast<long long>(per) * (blockIdx.x / p.lanes), static_cast<long long>(total)), left = min(per, total - u0);
   if (tid == 0) bar->start = {0, 0, 0, 0, 0, per};
   int before = 0;                                  // blocks of the sequences of earlier rounds
   for (int base = 0; base < p.batch; base += kThreads) {
@@ -113,7 +119,7 @@ __device__ __forceinline__ void find_start(const Params& p, Bars* bar) {
       cost = 0;
       if (b < p.batch) {
         q.load(p, b);
-        cost = p.kv_heads * q.template units_of_head<NT>(p);
+        cost = heads * q.template units_of_head<NT>(p);
       }
     }
     int incl = cost;
@@ -133,7 +139,7 @@ __device__ __forceinline__ void find_start(const Params& p, Bars* bar) {
     const int at = u0 - (offset + incl - cost);    // inside this thread's sequence?
     if (left > 0 && at >= 0 && at < cost) {
       q.load(p, b);
-      const int of_head = cost / p.kv_heads;
+      const int of_head = cost / heads;
       PagedStart s = {b, at / of_head, 0, at % of_head, left, per};
       for (int n; (n = q.template units<NT>(p, s.first_token)) <= s.block; s.first_token += NT * p.tile_tokens) s.block -= n;
       bar->start = s;
@@ -145,10 +151,15 @@ __device__ __forceinline__ void find_start(const Params& p, Bars* bar) {
 
 }  // namespace
 
-template <int D, bool BF16, int NT, bool PAGED, bool CAPPED, bool BIASED>
+template <int D, bool BF16, int NT, bool PAGED, bool CAPPED, bool BIASED, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __grid_constant__ Params p) {
-  using LO = Layout<D, NT>;
+  using LO = Layout<D, NT, SPLIT>;
+  static_assert(!SPLIT || (NT == 1 && PAGED), "four copies of an item's rows: single tokens");
   constexpr int kStages = LO::kStages, kAtoms = LO::kAtoms, kTile = LO::kTile;
+  constexpr bool kBiasProduct = BIASED && !CAPPED;
+  // Biased scores grow along a row, by 184 slope a block in units of the exponent: taken from the last block to the first, hardly a row has
+  // to move its reference, and its accumulator with it, more than once.
+  constexpr bool kBack = kBiasProduct;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars* bar = reinterpret_cast<Bars*>(smem + LO::kOffBar);
@@ -167,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       mbar_init(&bar->o_free[i], NT == 2 ? kSoftmaxWarps / 2 : kSoftmaxWarps);
     }
     mbar_init(&bar->sums_full, kSoftmaxWarps);
+    mbar_init(&bar->join_full, kSoftmaxWarps);
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&bar->seg_full[i], 1);
       mbar_init(&bar->seg_empty[i], kSoftmaxWarps + 2);
@@ -182,7 +194,6 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     tmem_alloc(&bar->tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  constexpr bool kBiasProduct = BIASED && !CAPPED;
   if constexpr (kBiasProduct) {
     uint8_t* bias = smem + LO::kOffBias;
     for (int i = threadIdx.x; i < kRows * 8; i += kThreads) {
@@ -222,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     int g = 0, segs = 0;
     uint32_t loads_q = 0;                          // parities, a bit a tile
     bool ok = true;
-    const uint32_t q_bytes = static_cast<uint32_t>(p.group * p.tile_tokens) * 128 * kAtoms;
+    const uint32_t q_bytes = static_cast<uint32_t>(p.group * p.tile_tokens) * 128 * kAtoms * (SPLIT ? 4 : 1);
     bool more = true;
     while (ok && more) {
       do {
@@ -249,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         if constexpr (kBiasProduct) {
           const bool brought = p.bias_product && keys_in_front(p, s, t);
           for (int row = lane; row < kRows; row += 32) {
-            const float slope = brought ? p.slopes[s.kv_head * p.group + row % p.group] * p.bias_unit : 0.f;
+            const float slope = brought ? p.slopes[s.kv_head * p.group + (SPLIT ? row % 32 : row) % p.group] * p.bias_unit : 0.f;
             *reinterpret_cast<uint2*>(bias_at(smem + LO::kOffBias, row, 2 * t)) = bias_terms(slope);
           }
           fence_proxy_async_smem();
@@ -257,13 +268,15 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         }
         if (lane == 0) {
           mbar_arrive_expect_tx(&bar->q_full[t], q_bytes);
-          for (int a = 0; a < kAtoms; ++a)
-            tma_load_4d(smem + t * kTile + a * (kRows * 128), &p.map_q, &bar->q_full[t], a * 64, s.kv_head * p.group,
+          for (int copy = 0; copy < (SPLIT ? 4 : 1); ++copy)
+           for (int a = 0; a < kAtoms; ++a)
+            tma_load_4d(smem + t * kTile + a * (kRows * 128) + copy * (32 * 128), &p.map_q, &bar->q_full[t], a * 64, s.kv_head * p.group,
                         s.row0 + s.first_token + t * p.tile_tokens, PAGED ? 0 : s.seq);
         }
         __syncwarp();
       }
-      for (int j = s.begin(); ok && j < s.end(); ++j) {
+      for (int i = s.begin(); ok && i < s.end(); ++i) {
+        const int j = s.template block<kBack>(i);
         // rows of this block that pages bring: lane i loads page i of the block
         int page = -1, rows = kKeys, lanes = 1, row_in_page = 0;
         if constexpr (PAGED) {
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       ok = wait(&bar->seg_full[slot], (segs / kSegs) & 1, 0x350);
       if (!ok || !segments[slot].valid) break;
       const int begin = segments[slot].begin(), end = segments[slot].end(), block0 = segments[slot].block0 - begin;
-      const int first = segments[slot].lo(t) + (NT == 1 ? buf : 0), last = segments[slot].hi(t);
+      const int first = segments[slot].template first_step<kBack>(t) + (NT == 1 ? buf : 0), last = segments[slot].template last_step<kBack>(t);
       if (begin >= end) {
         mbar_arrive_warp(&bar->seg_empty[slot], lane);
         continue;
@@ -433,11 +446,15 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t s_col = lane_base + buf * kKeys, o_col = lane_base + kColO;
     float2* sums = reinterpret_cast<float2*>(smem + LO::kOffSum) + row;
-    const int r_token = row / p.group, r_head = row - r_token * p.group;
+    const int in_copy = SPLIT ? lane : row, r_token = in_copy / p.group, r_head = in_copy - r_token * p.group;
+    // this thread's keys of a block
+    constexpr int kMine = SPLIT ? 32 : kKeys;
+    const int my_keys = SPLIT ? quad * 32 : 0;
     const bool row_used = r_token < p.tile_tokens;
     const float c = p.c;
     const int t = NT == 2 ? buf : 0;
     int n = 0, segs = 0;
+    [[maybe_unused]] int joins = 0;
     uint32_t done = 0;
     bool ok = true;
     if constexpr (PAGED) {
@@ -474,14 +491,15 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       RowReference ref(c);
       if (limit == 0) ref.m = 0.f, ref.large = false;      // sees nothing: asks for no rescale
       float l = 0.f;
-      const int first = s.lo(t) + (NT == 1 ? buf : 0), end = s.hi(t);
-      for (int j = first; j < end; j += NT == 1 ? 2 : 1) {
+      const int first = s.template first_step<kBack>(t) + (NT == 1 ? buf : 0), end = s.template last_step<kBack>(t);
+      for (int step = first; step < end; step += NT == 1 ? 2 : 1) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[buf], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
-        uint32_t sv[kKeys];
-        tmem_ld_x128_wait(s_col, sv);
-        const int k0 = j * kKeys;
+        uint32_t sv[kMine];
+        if constexpr (SPLIT) tmem_ld_x32_wait(s_col + my_keys, sv);
+        else tmem_ld_x128_wait(s_col, sv);
+        const int j = s.template block<kBack>(step), k0 = j * kKeys + my_keys;
         float base = 0.f;                              // what the row's scores in sv lack
         if (CAPPED && p.cap_out != 0.f) {
           capped(sv, p.cap_in, p.cap_out);
@@ -503,22 +521,22 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         if (j >= cut) {
           const int lim = limit - k0;
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
+          for (int i = 0; i < kMine; ++i)
             if (i >= lim) sv[i] = __float_as_uint(-INFINITY);
         }
         if (!PAGED && cut_low > k0) {
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
+          for (int i = 0; i < kMine; ++i)
             if (i < low - k0) sv[i] = __float_as_uint(-INFINITY);
         }
         float mx[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) mx[u] = __uint_as_float(sv[u]);
 #pragma unroll
-        for (int i = 8; i < kKeys; i += 16) {
+        for (int i = 8; i < kMine; i += 16) {
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            if (i + 8 < kKeys) mx[u] = max3(mx[u], __uint_as_float(sv[i + u]), __uint_as_float(sv[i + 8 + u]));
+            if (i + 8 < kMine) mx[u] = max3(mx[u], __uint_as_float(sv[i + u]), __uint_as_float(sv[i + 8 + u]));
             else mx[u] = fmaxf(mx[u], __uint_as_float(sv[i + u]));
           }
         }
@@ -527,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         const bool need = ref.asks(m_new, c, kRescaleThreshold) && m_new != -INFINITY;
         if (__any_sync(0xffffffffu, need)) {
           const float f = ref.move(m_new, c);
-          if (j != first) {                        // (these scores were issued behind the P V of the buffer's last step: O is quiet)
+          if (step != first) {                      // (these scores were issued behind the P V of the buffer's last step: O is quiet)
 #pragma unroll
             for (int cc = 0; cc < D; cc += 16) {
               uint32_t o[16];
@@ -541,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           l *= f;
           if (kBiasProduct && __any_sync(0xffffffffu, ref.large && base != 0.f)) {
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) + base);
+            for (int i = 0; i < kMine; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) + base);
             base = 0.f;
           }
           ref.subtract(sv);
@@ -549,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         if constexpr (PAGED) {
           // the slots behind a sequence's end hold anything: their values become zeros, which their weights, zeros too, need
           if ((j + 1) * kKeys > s.keys) {      // (with two tiles both do this, and write the same)
-            const int nv = 2 * (s.block0 + j - s.begin()) + 1, st = nv % kStages;
+            const int nv = 2 * (s.block0 + step - s.begin()) + 1, st = nv % kStages;
             ok = __all_sync(0xffffffffu, mbar_wait(&bar->kv_full[st], (nv / kStages) & 1, abort_word, 0x820));
             if (!ok) break;
             uint8_t* v = smem + LO::kOffKV + st * kTile;
@@ -562,25 +580,41 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         const float mc = kBiasProduct ? fmaf(-base, c, ref.offset(c)) : ref.offset(c);
         const uint64_t c2 = pack_f32x2(c, c), nmc2 = pack_f32x2(-mc, -mc);
         uint64_t sum2[2] = {0, 0};
+        auto weights_of = [&](uint32_t (&pk)[16], int pair0) {
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-#pragma unroll
-          for (int chunk = part == 0 ? 0 : kSplit / 32; chunk < (part == 0 ? kSplit : kKeys) / 32; ++chunk) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int pair = chunk * 16 + i;
-              const uint64_t weights = softmax_weights(sv[2 * pair], sv[2 * pair + 1], c2, nmc2, weights_on_fma(pair));
-              sum2[i & 1] = add_f32x2(sum2[i & 1], weights);
-              float p0, p1;
-              unpack_f32x2(weights, p0, p1);
-              pk[i] = pack2<BF16>(p0, p1);
-            }
-            tmem_st_x16(s_col + chunk * 16, pk);
+          for (int i = 0; i < 16; ++i) {
+            const int pair = pair0 + i;
+            const uint64_t weights = softmax_weights(sv[2 * pair], sv[2 * pair + 1], c2, nmc2, weights_on_fma(pair));
+            sum2[i & 1] = add_f32x2(sum2[i & 1], weights);
+            float p0, p1;
+            unpack_f32x2(weights, p0, p1);
+            pk[i] = pack2<BF16>(p0, p1);
           }
+        };
+        if constexpr (SPLIT) {
+          // the keys of the other warps have no weight in this warp's copy of the rows
+          uint32_t pk[16], none[16] = {};
+          weights_of(pk, 0);
+#pragma unroll
+          for (int other = 1; other < 4; ++other) tmem_st_x16(s_col + ((quad + other) & 3) * 16, none);
+          tmem_st_x16(s_col + quad * 16, pk);
           tmem_wait_st();
           tc_fence_before_sync();
-          mbar_arrive_warp(&bar->p_part[buf][part], lane);
+          mbar_arrive_warp(&bar->p_part[buf][0], lane);
+          mbar_arrive_warp(&bar->p_part[buf][1], lane);
+        } else {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+#pragma unroll
+            for (int chunk = part == 0 ? 0 : kSplit / 32; chunk < (part == 0 ? kSplit : kKeys) / 32; ++chunk) {
+              uint32_t pk[16];
+              weights_of(pk, chunk * 16);
+              tmem_st_x16(s_col + chunk * 16, pk);
+            }
+            tmem_wait_st();
+            tc_fence_before_sync();
+            mbar_arrive_warp(&bar->p_part[buf][part], lane);
+          }
         }
         float s0, s1;
         unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
@@ -603,12 +637,27 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         mbar_arrive_warp(&bar->sums_full, lane);
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->sums_full, segs & 1, abort_word, 0x850));
         if (!ok) break;
-        const float2 other = both[(buf ^ 1) * 128];
-        const float m = other.y == 0.f ? ref.m : l == 0.f ? other.x : fmaxf(ref.m, other.x);
-        f_mine = ref.m == m ? 1.0f : l == 0.f ? 0.f : ex2_approx((ref.m - m) * c);
-        f_other = other.y == 0.f ? 0.f : other.x == m ? 1.0f : ex2_approx((other.x - m) * c);
-        l = l * f_mine + other.y * f_other;
-        ref.m = m;
+        if constexpr (SPLIT) {
+          const float2* all = both - row + lane;       // of the row's eight threads: buffer, copy
+          float m = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (all[i * 32].y != 0.f) m = fmaxf(m, all[i * 32].x);
+          auto factor = [&](float2 ml) { return ml.y == 0.f ? 0.f : ml.x == m ? 1.0f : ex2_approx((ml.x - m) * c); };
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum = fmaf(all[i * 32].y, factor(all[i * 32]), sum);
+          f_mine = factor(make_float2(ref.m, l));
+          f_other = factor(both[(buf ^ 1) * 128]);
+          l = sum;
+          ref.m = m;
+        } else {
+          const float2 other = both[(buf ^ 1) * 128];
+          const float m = other.y == 0.f ? ref.m : l == 0.f ? other.x : fmaxf(ref.m, other.x);
+          f_mine = ref.m == m ? 1.0f : l == 0.f ? 0.f : ex2_approx((ref.m - m) * c);
+          f_other = other.y == 0.f ? 0.f : other.x == m ? 1.0f : ex2_approx((other.x - m) * c);
+          l = l * f_mine + other.y * f_other;
+          ref.m = m;
+        }
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -619,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       if (!ok) break;
       tc_fence_after_sync();
       const float inv = s.part >= 0 ? 1.0f : l == 0.f ? 0.f : 1.0f / l;
-      const size_t part_at = PAGED && s.part >= 0 ? ((static_cast<size_t>(blockIdx.x) * 2 + s.part) * NT + t) * kRows + row : 0;
+      const size_t part_at = PAGED && s.part >= 0 ? ((static_cast<size_t>(blockIdx.x) * 2 + s.part) * NT + t) * (SPLIT ? 32 : kRows) + in_copy : 0;
       uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) +
                      2 * ((PAGED ? 0 : s.seq * p.out_batch) + (s.row0 + static_cast<long long>(token)) * p.out_token + head * p.out_head);
 #pragma unroll
@@ -646,6 +695,30 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           for (int b = 0; b < 2; ++b)
             if ((NT == 1 || b == buf) && has[b]) mbar_arrive_warp(&bar->o_free[b], lane);
         }
+        if constexpr (SPLIT) {
+          // the sum over the four copies: a warp takes four columns of a row each from the other warps of its buffer's half of the columns
+          float* join = reinterpret_cast<float*>(smem + LO::kOffJoin) + (joins & 1) * (kSoftmaxWarps * 512) + buf * 2048;
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(join + (quad * 32 + lane) * 16 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          mbar_arrive_warp(&bar->join_full, lane);
+          ok = __all_sync(0xffffffffu, mbar_wait(&bar->join_full, joins & 1, abort_word, 0x860));
+          if (!ok) break;
+          ++joins;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int copy = 0; copy < 4; ++copy) {
+            const float4 y = *reinterpret_cast<const float4*>(join + (copy * 32 + lane) * 16 + quad * 4);
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+          }
+          const int col = col0 + cc + quad * 4;
+          if (valid && s.part >= 0) {
+            if (l != 0.f) *reinterpret_cast<float4*>(p.part_o + part_at * D + col) = x;
+          } else if (valid && col < p.d) {
+            *reinterpret_cast<uint2*>(dst + 2 * col) =
+                l == 0.f ? make_uint2(0, 0) : make_uint2(pack2<BF16>(x.x * inv, x.y * inv), pack2<BF16>(x.z * inv, x.w * inv));
+          }
+          continue;
+        }
         if (!valid) continue;
         if (PAGED && s.part >= 0) {
           if (l != 0.f) {
@@ -663,7 +736,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           if (col0 + cc + i < p.d) *reinterpret_cast<uint4*>(dst + 2 * (col0 + cc + i)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
-      if (valid && (NT == 2 || buf == 0)) {
+      if (!ok) break;
+      if (valid && (NT == 2 || buf == 0) && (!SPLIT || quad == 0)) {
         if (PAGED && s.part >= 0) p.part_ml[part_at] = make_float2(l == 0.f ? -INFINITY : ref.m, l);
         if (!PAGED && p.lse != nullptr)
           p.lse[(static_cast<size_t>(s.seq) * p.M + token) * p.heads + head] = l == 0.f ? -INFINITY : fmaf(ref.m * c, kLn2, logf(l));
@@ -671,8 +745,10 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       if constexpr (PAGED) {
         if (s.part == 1 && threadIdx.x == 0) {
           // this CTA began the item: its parts end with the CTA whose share holds the item's last block
-          const long long first_unit = static_cast<long long>(blockIdx.x) * bar->start.per_cta + s.at_unit;
-          p.parts[blockIdx.x] = {s.seq, s.kv_head, s.first_token, static_cast<int>((first_unit + s.units - 1) / bar->start.per_cta)};
+          const int share = blockIdx.x / p.lanes;
+          const long long first_unit = static_cast<long long>(share) * bar->start.per_cta + s.at_unit;
+          const int last_share = static_cast<int>((first_unit + s.units - 1) / bar->start.per_cta);
+          p.parts[blockIdx.x] = {s.seq, s.kv_head, s.first_token, static_cast<int>(blockIdx.x) + (last_share - share) * p.lanes};
         }
       }
       mbar_arrive_warp(&bar->seg_empty[slot], lane);
@@ -693,22 +769,22 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
 
 namespace {
 
-template <int D, bool BF16, int NT, bool PAGED, bool CAPPED, bool BIASED>
+template <int D, bool BF16, int NT, bool PAGED, bool CAPPED, bool BIASED, bool SPLIT = false>
 cudaError_t launch_one(const Params& p, int grid, cudaStream_t stream) {
-  auto kern = masked_forward_kernel<D, BF16, NT, PAGED, CAPPED, BIASED>;
+  auto kern = masked_forward_kernel<D, BF16, NT, PAGED, CAPPED, BIASED, SPLIT>;
   static std::atomic<unsigned long long> configured{0};
   int dev = 0;
   cudaError_t e = current_device_checked(&dev);
   if (e != cudaSuccess) return e;
   if (!device_configured(configured, dev)) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D, NT>::kBytes);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D, NT, SPLIT>::kBytes);
     if (e != cudaSuccess) return e;
     mark_device_configured(configured, dev);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = Layout<D, NT>::kBytes;
+  cfg.dynamicSmemBytes = Layout<D, NT, SPLIT>::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -723,6 +799,9 @@ cudaError_t launch_one(const Params& p, int grid, cudaStream_t stream) {
 namespace {
 template <int D, bool BF16, bool PAGED, bool CAPPED, bool BIASED>
 cudaError_t launch_tiles(const Params& p, int tiles, int grid, cudaStream_t stream) {
+  if constexpr (PAGED) {
+    if (tiles == 0) return launch_one<D, BF16, 1, PAGED, CAPPED, BIASED, true>(p, grid, stream);
+  }
   return tiles == 2 ? launch_one<D, BF16, 2, PAGED, CAPPED, BIASED>(p, grid, stream) : launch_one<D, BF16, 1, PAGED, CAPPED, BIASED>(p, grid, stream);
 }
 }  // namespace

@@ -171,13 +171,13 @@ __global__ void __launch_bounds__(kSumThreads) sum_parts_kernel(const __grid_con
   grid_launch_dependents();
   const PartDesc part = p.parts[blockIdx.x];
   if (part.last_cta < 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = part.last_cta - static_cast<int>(blockIdx.x) + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (part.last_cta - static_cast<int>(blockIdx.x)) / p.lanes + 1;
   Sequence q;
   q.load(p, part.seq);
   for (int r = blockIdx.y + kSumSlices * warp; r < rows; r += kSumSlices * (kSumThreads / 32)) {
     const int in_tile = r % kRows, token = part.first_token + (r / kRows) * p.tile_tokens + in_tile / p.group;
     if (in_tile / p.group >= p.tile_tokens || token >= q.tokens) continue;
-    auto at = [&](int i) { return (static_cast<size_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * rows + r; };
+    auto at = [&](int i) { return (static_cast<size_t>(blockIdx.x + i * p.lanes) * 2 + (i == 0 ? 1 : 0)) * rows + r; };
     float m = -INFINITY;
     for (int i = lane; i < n; i += 32) m = fmaxf(m, p.part_ml[at(i)].x);
 #pragma unroll
@@ -238,7 +238,7 @@ cudaError_t launch_document_plan(const int* documents, const int* prefix, int ba
 cudaError_t launch_sum_parts(const Params& p, int d, bool bf16, int tiles, int grid, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = config(grid, kSumThreads, stream, attr, kSumSlices);
-  const int rows = tiles * kRows;
+  const int rows = tiles == 0 ? 32 : tiles * kRows;
   if (d == 128) return bf16 ? launch_kernel(cfg, sum_parts_kernel<128, true>, p, rows) : launch_kernel(cfg, sum_parts_kernel<128, false>, p, rows);
   return bf16 ? launch_kernel(cfg, sum_parts_kernel<64, true>, p, rows) : launch_kernel(cfg, sum_parts_kernel<64, false>, p, rows);
 }

@@ -57,6 +57,7 @@ struct Params {
   const int* starts;          // [batch + 1], or null: a token a sequence
   long long table_stride;
   int page, pages;
+  int lanes;                  // key heads that are worked on side by side: CTA x has heads x % lanes, + lanes, ... of its share of the blocks
   float* part_o;              // [CTA][2][tiles of an item x 128][D]
   float2* part_ml;            // [CTA][2][tiles of an item x 128]: reference (in scores) and sum
   PartDesc* parts;            // [CTA]
@@ -81,6 +82,13 @@ struct Segment {
 
   __device__ __forceinline__ int lo(int t) const { return NT == 1 || t == 0 ? lo0 : lo1; }
   __device__ __forceinline__ int hi(int t) const { return NT == 1 || t == 0 ? hi0 : hi1; }
+  // Blocks in the order in which they are taken: step i takes block i, or, from the last to the first, block begin + end - 1 - i.
+  template <bool BACK>
+  __device__ __forceinline__ int block(int i) const { return BACK ? begin() + end() - 1 - i : i; }
+  template <bool BACK>
+  __device__ __forceinline__ int first_step(int t) const { return BACK ? begin() + end() - hi(t) : lo(t); }
+  template <bool BACK>
+  __device__ __forceinline__ int last_step(int t) const { return BACK ? begin() + end() - lo(t) : hi(t); }
   __device__ __forceinline__ void set(int t, int lo, int hi) {
     if (t == 0) lo0 = lo, hi0 = hi;
     else lo1 = lo, hi1 = hi;
@@ -168,7 +176,8 @@ struct Sequence {
   }
 };
 
-// Where a CTA begins in the sequence (sequence, key head, tiles, block) of all blocks, and how many it has; per_cta is everybody's share.
+// Where a CTA begins in the order (sequence, key head of its lane, tiles, block) of its lane's blocks, and how many it has; per_cta is everybody's
+// share.  kv_head counts the heads of the lane.
 struct PagedStart {
   int seq, kv_head, first_token, block, left, per_cta;
 };
@@ -184,7 +193,7 @@ struct PagedWalker {
     q.load(p, at.seq);
     while (at.first_token >= q.tokens) {        // the next key head, the next sequence with tokens
       at.first_token = 0;
-      if (q.tokens == 0 || ++at.kv_head == p.kv_heads) {
+      if (q.tokens == 0 || ++at.kv_head == p.kv_heads / p.lanes) {
         at.kv_head = 0;
         if (++at.seq >= p.batch) return false;
         q.load(p, at.seq);
@@ -192,7 +201,7 @@ struct PagedWalker {
     }
     const int units = q.units<NT>(p, at.first_token), take = min(at.left, units - at.block);
     s.seq = at.seq;
-    s.kv_head = at.kv_head;
+    s.kv_head = at.kv_head * p.lanes + static_cast<int>(blockIdx.x) % p.lanes;
     s.first_token = at.first_token;
     s.tokens = q.tokens;
     s.keys = q.keys;
