@@ -496,15 +496,29 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[buf], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
+        const int j = s.template block<kBack>(step), k0 = j * kKeys + my_keys;
+        auto modified = [&](uint32_t (&part)[32], int at) {
+          capped(part, p.cap_in, p.cap_out);
+          if (p.slopes != nullptr) biased(part, 1.0f, slope, static_cast<float>(pos - at), in_front);
+        };
+        if constexpr (CAPPED && !SPLIT) {
+          // a quarter of the scores at a time and back to where they were: with a whole row of them there are no registers for this
+#pragma unroll 1
+          for (int i = 0; i < kMine; i += 32) {
+            uint32_t part[32];
+            tmem_ld_x32_wait(s_col + i, part);
+            modified(part, k0 + i);
+            tmem_st_x16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(&part[0]));
+            tmem_st_x16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(&part[16]));
+          }
+          tmem_wait_st();
+        }
         uint32_t sv[kMine];
         if constexpr (SPLIT) tmem_ld_x32_wait(s_col + my_keys, sv);
         else tmem_ld_x128_wait(s_col, sv);
-        const int j = s.template block<kBack>(step), k0 = j * kKeys + my_keys;
+        if constexpr (CAPPED && SPLIT) modified(sv, k0);
         float base = 0.f;                              // what the row's scores in sv lack
-        if (CAPPED && p.cap_out != 0.f) {
-          capped(sv, p.cap_in, p.cap_out);
-          if (p.slopes != nullptr) biased(sv, 1.0f, slope, static_cast<float>(pos - k0), in_front);
-        } else if (BIASED) {
+        if constexpr (kBiasProduct) {
           if (brought) base = slope * static_cast<float>(k0 - pos);
           else biased(sv, p.bias_factor, slope, static_cast<float>(pos - k0), in_front);
         }
