@@ -34,7 +34,7 @@ constexpr uint32_t kTmemCols = 512, kColO = 256;
 constexpr float kRescaleThreshold = 8.0f;     // log2 units by which a row's maximum may run ahead of its reference
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kSegs = 4;                      // items that the producer is ahead of the others
-constexpr int kSplit = 96;                    // keys in the first part of P: their P V runs under the last exponentials
+constexpr int kHalfKeys = kKeys / 2;
 
 // SPLIT: items of a single token, whose heads (32 at most) fill a part of a tile only.  Four copies of the rows, at rows 0, 32, 64 and 96: a warp has
 // a quarter of a block's keys of each row instead of a thread a whole row, and no weight on the others; the copies' results are summed at an item's
@@ -57,9 +57,9 @@ struct Layout {
 struct Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[8], kv_empty[8];
-  uint64_t s_full[2], p_part[2][2], o_done[2], o_free[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], o_done[2], o_free[2];      // [buffer][half]
   uint64_t seg_full[kSegs], seg_empty[kSegs];
-  uint64_t turn[2], sums_full, join_full;
+  uint64_t sums_full, join_full;
   uint32_t tmem_base, abort_word;
   PagedStart start;
   int scan[kThreads / 32 + 1];
@@ -170,11 +170,12 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->q_full[i], 1);
       mbar_init(&bar->q_empty[i], NT == 2 ? 1 : 2);
-      mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->p_part[i][0], kSoftmaxWarps / 2);
-      mbar_init(&bar->p_part[i][1], kSoftmaxWarps / 2);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bar->s_full[i][h], 1);
+        mbar_init(&bar->p_full[i][h], kSoftmaxWarps / 2);
+      }
+      mbar_init(&bar->pv_done[i], 1);
       mbar_init(&bar->o_done[i], 1);
-      mbar_init(&bar->turn[i], 1);
       mbar_init(&bar->o_free[i], NT == 2 ? kSoftmaxWarps / 2 : kSoftmaxWarps);
     }
     mbar_init(&bar->sums_full, kSoftmaxWarps);
@@ -318,12 +319,12 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     // ------------------------------------------------------------ MMA issuer of a buffer (converged warp, elected lane issues)
     const int buf = warp - kMmaWarp, t = NT == 2 ? buf : 0;
     const uint32_t issuer = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kKeys, false, false);
+    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kHalfKeys, false, false);
     const uint32_t idesc_o = umma_idesc_f16(BF16, kRows, D, false, true);
     const uint64_t dq = umma_desc_sw128(smem_u32(smem + t * kTile), 16, 1024);
     const uint64_t dk0 = umma_desc_sw128(smem_u32(smem + LO::kOffKV), 16, 1024);
     const uint64_t dv0 = umma_desc_sw128(smem_u32(smem + LO::kOffKV), kKeys * 128, 1024);
-    [[maybe_unused]] const uint32_t idesc_bias = umma_idesc_f16(true, kRows, kKeys, false, false);
+    [[maybe_unused]] const uint32_t idesc_bias = umma_idesc_f16(true, kRows, kHalfKeys, false, false);
     [[maybe_unused]] const uint64_t dbias = umma_desc_sw128(smem_u32(smem + LO::kOffBias), 16, 1024);
     const uint32_t d_o = tmem_base + kColO + buf * D, d_s = tmem_base + buf * kKeys;
     auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
@@ -338,27 +339,19 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       return r;
     };
     auto wait_kv = [&](int n) { return wait(&bar->kv_full[n % kStages], (n / kStages) & 1, 0x310); };      // n: 2 block, or 2 block + 1
-    auto issue_s = [&](int block) {
+    auto issue_s = [&](int block, int h) {
       const int st = (2 * block) % kStages;
-      const uint64_t db = dk0 + ((st * kTile) >> 4);
+      const uint64_t db = dk0 + ((st * kTile + h * (kHalfKeys * 128)) >> 4);
+      const uint32_t d = d_s + h * kHalfKeys;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
-        umma_ss_elected(d_s, dq + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
+        umma_ss_elected(d, dq + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
       }
-      if constexpr (kBiasProduct) umma_ss_elected(d_s, dbias + 2 * t, dbias + 4, idesc_bias, 1u, issuer);
-      umma_commit_elected(&bar->s_full[buf], issuer);
-      umma_commit_elected(&bar->kv_empty[st], issuer);
+      if constexpr (kBiasProduct) umma_ss_elected(d, dbias + 2 * t, dbias + 4 + ((h * (kHalfKeys * 128)) >> 4), idesc_bias, 1u, issuer);
+      umma_commit_elected(&bar->s_full[buf][h], issuer);
+      if (h == 1) umma_commit_elected(&bar->kv_empty[st], issuer);
     };
-    // The buffers take turns, block by block: one's P V and next scores, then the other's.  Mixed, both buffers' scores would be ready at
-    // the same time, and from then on both would have their exponentials, and both their MMAs, at the same time.
-    uint32_t turns = 0;
-    auto take_turn = [&]() {
-      const bool r = wait(&bar->turn[buf], (turns & 1) ^ (buf == 0 ? 1u : 0u), 0x360);
-      ++turns;
-      return r;
-    };
-    auto give_turn = [&]() { mbar_arrive_warp(&bar->turn[buf ^ 1], lane); };
     constexpr int kStep = NT == 2 ? 1 : 2;
     uint32_t loads_q = 0, uses_o = 0, n = 0;           // tiles and accumulators so far, steps so far
     bool ok = true;
@@ -378,8 +371,6 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           if (!wait_kv(2 * (block0 + j) + kv)) return false;
           mbar_arrive_warp(&bar->kv_empty[(2 * (block0 + j) + kv) % kStages], lane);
         }
-        if (!take_turn()) return false;
-        give_turn();
         return true;
       };
       if constexpr (NT == 2) {
@@ -393,7 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       if (first < last) {
         ok = wait_kv(2 * (block0 + first));
         if (!ok) break;
-        issue_s(block0 + first);
+        issue_s(block0 + first, 0);
+        issue_s(block0 + first, 1);
       }
       mbar_arrive_warp(&bar->seg_empty[slot], lane);
       if (first + kStep >= last) {                     // Q has been read with the item's last scores
@@ -415,29 +407,31 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           ++uses_o;
         }
         const uint64_t db = dv0 + ((sv * kTile) >> 4);
-        if (!(ok = wait_both(&bar->turn[buf], (turns & 1) ^ (buf == 0 ? 1u : 0u), &bar->p_part[buf][0], n & 1, 0x340))) break;
-        ++turns;
+        auto issue_pv = [&](int h) {
 #pragma unroll
-        for (int i = 0; i < kSplit / 16; ++i)
-          umma_ts_elected(d_o, d_s + i * 8, db + ((i * 2048) >> 4), idesc_o, i > 0 || j > first ? 1u : 0u, issuer);
-        if (!(ok = wait(&bar->p_part[buf][1], n & 1, 0x341))) break;
-#pragma unroll
-        for (int i = kSplit / 16; i < kKeys / 16; ++i) umma_ts_elected(d_o, d_s + i * 8, db + ((i * 2048) >> 4), idesc_o, 1u, issuer);
+          for (int i = 0; i < kHalfKeys / 16; ++i)
+            umma_ts_elected(d_o, d_s + h * kHalfKeys + i * 8, db + (((h * (kHalfKeys / 16) + i) * 2048) >> 4), idesc_o, i > 0 || h > 0 || j > first ? 1u : 0u, issuer);
+          umma_commit_elected(&bar->pv_done[buf], issuer);
+        };
+        if (!(ok = wait(&bar->p_full[buf][0], n & 1, 0x340))) break;
+        issue_pv(0);
+        if (NT == 2 && next < last) issue_s(block0 + next, 0);
+        if (!(ok = wait(&bar->p_full[buf][1], n & 1, 0x341))) break;
+        issue_pv(1);
         umma_commit_elected(&bar->kv_empty[sv], issuer);
         if (next < last) {
-          if (NT == 1 && !(ok = wait_kv(2 * (block0 + next)))) break;
-          issue_s(block0 + next);
+          if (NT == 1) {
+            if (!(ok = wait_kv(2 * (block0 + next)))) break;
+            issue_s(block0 + next, 0);
+          }
+          issue_s(block0 + next, 1);
           if (next + kStep >= last) umma_commit_elected(&bar->q_empty[t], issuer);
         } else {
           umma_commit_elected(&bar->o_done[buf], issuer);
         }
-        give_turn();
       }
       if constexpr (NT == 2) {
         for (int j = max(begin, max(last, min(first, end))); ok && j < end; ++j) ok = pass(j);
-      } else if (buf == 1 && ((end - begin) & 1)) {      // the last turn of an odd number of blocks
-        ok = ok && take_turn();
-        give_turn();
       }
     }
   } else {
@@ -448,8 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     float2* sums = reinterpret_cast<float2*>(smem + LO::kOffSum) + row;
     const int in_copy = SPLIT ? lane : row, r_token = in_copy / p.group, r_head = in_copy - r_token * p.group;
     // this thread's keys of a block
-    constexpr int kMine = SPLIT ? 32 : kKeys;
-    const int my_keys = SPLIT ? quad * 32 : 0;
+    constexpr int kMine = SPLIT ? 32 : kHalfKeys, kParts = SPLIT ? 1 : 2;
     const bool row_used = r_token < p.tile_tokens;
     const float c = p.c;
     const int t = NT == 2 ? buf : 0;
@@ -486,53 +479,45 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       }
       const float slope = BIASED && p.slopes != nullptr && valid ? p.slopes[head] * (CAPPED ? 1.4426950408889634f : p.bias_unit) : 0.f;
       // the first block that a row of this warp does not see whole, and the last one in which one does not see the first key (documents)
-      const int cut = __reduce_min_sync(0xffffffffu, limit) / kKeys, cut_low = __reduce_max_sync(0xffffffffu, low);
+      const int cut = __reduce_min_sync(0xffffffffu, limit), cut_low = __reduce_max_sync(0xffffffffu, low);
       const bool in_front = keys_in_front(p, s, t), brought = kBiasProduct && p.bias_product && in_front;
       RowReference ref(c);
       if (limit == 0) ref.m = 0.f, ref.large = false;      // sees nothing: asks for no rescale
       float l = 0.f;
       const int first = s.template first_step<kBack>(t) + (NT == 1 ? buf : 0), end = s.template last_step<kBack>(t);
-      for (int step = first; step < end; step += NT == 1 ? 2 : 1) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[buf], n & 1, abort_word, 0x800));
+      for (int step = first; ok && step < end; step += NT == 1 ? 2 : 1, ++n) {
+#pragma unroll 1
+       for (int h = 0; h < kParts; ++h) {
+        const int part0 = SPLIT ? quad * 32 : h * kHalfKeys;       // this thread's keys of the block begin there
+        ok = SPLIT ? mbar_wait(&bar->s_full[buf][0], n & 1, abort_word, 0x800) && mbar_wait(&bar->s_full[buf][1], n & 1, abort_word, 0x801)
+                   : mbar_wait(&bar->s_full[buf][h], n & 1, abort_word, 0x800);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after_sync();
-        const int j = s.template block<kBack>(step), k0 = j * kKeys + my_keys;
-        auto modified = [&](uint32_t (&part)[32], int at) {
-          capped(part, p.cap_in, p.cap_out);
-          if (p.slopes != nullptr) biased(part, 1.0f, slope, static_cast<float>(pos - at), in_front);
-        };
-        if constexpr (CAPPED && !SPLIT) {
-          // a quarter of the scores at a time and back to where they were: with a whole row of them there are no registers for this
-#pragma unroll 1
-          for (int i = 0; i < kMine; i += 32) {
-            uint32_t part[32];
-            tmem_ld_x32_wait(s_col + i, part);
-            modified(part, k0 + i);
-            tmem_st_x16(s_col + i, *reinterpret_cast<uint32_t(*)[16]>(&part[0]));
-            tmem_st_x16(s_col + i + 16, *reinterpret_cast<uint32_t(*)[16]>(&part[16]));
-          }
-          tmem_wait_st();
-        }
+        const int j = s.template block<kBack>(step), k0 = j * kKeys + part0;
         uint32_t sv[kMine];
-        if constexpr (SPLIT) tmem_ld_x32_wait(s_col + my_keys, sv);
-        else tmem_ld_x128_wait(s_col, sv);
-        if constexpr (CAPPED && SPLIT) modified(sv, k0);
+        if constexpr (SPLIT) tmem_ld_x32_wait(s_col + part0, sv);
+        else tmem_ld_x64_wait(s_col + part0, sv);
         float base = 0.f;                              // what the row's scores in sv lack
+        if constexpr (CAPPED) {
+          capped(sv, p.cap_in, p.cap_out);
+          if (p.slopes != nullptr) biased(sv, 1.0f, slope, static_cast<float>(pos - k0), in_front);
+        }
         if constexpr (kBiasProduct) {
-          if (brought) base = slope * static_cast<float>(k0 - pos);
+          if (brought) base = slope * static_cast<float>(j * kKeys - pos);
           else biased(sv, p.bias_factor, slope, static_cast<float>(pos - k0), in_front);
         }
         if constexpr (!PAGED) {
           if (mixed) {
             const int* ids = p.documents + static_cast<size_t>(s.seq) * p.L;
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
+            for (int i = 0; i < kMine; ++i) {
               if (ids[min(k0 + i, p.L - 1)] != doc) sv[i] = __float_as_uint(-INFINITY);
               if (i % 8 == 7) asm volatile("" ::: "memory");       // (eight ids at a time: registers)
             }
           }
         }
-        if (j >= cut) {
+        if (k0 + kMine > cut) {
           const int lim = limit - k0;
 #pragma unroll
           for (int i = 0; i < kMine; ++i)
@@ -559,7 +544,13 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         const bool need = ref.asks(m_new, c, kRescaleThreshold) && m_new != -INFINITY;
         if (__any_sync(0xffffffffu, need)) {
           const float f = ref.move(m_new, c);
-          if (step != first) {                      // (these scores were issued behind the P V of the buffer's last step: O is quiet)
+          if (step != first || h > 0) {
+            // one P V at most is under way, the last half's: the one before was issued ahead of these scores
+            if constexpr (!SPLIT) {
+              ok = __all_sync(0xffffffffu, mbar_wait(&bar->pv_done[buf], h ^ 1, abort_word, 0x810));
+              if (!ok) break;
+              tc_fence_after_sync();
+            }
 #pragma unroll
             for (int cc = 0; cc < D; cc += 16) {
               uint32_t o[16];
@@ -580,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         }
         if constexpr (PAGED) {
           // the slots behind a sequence's end hold anything: their values become zeros, which their weights, zeros too, need
-          if ((j + 1) * kKeys > s.keys) {      // (with two tiles both do this, and write the same)
+          if (h == 0 && (j + 1) * kKeys > s.keys) {      // (with two tiles both do this, and write the same)
             const int nv = 2 * (s.block0 + step - s.begin()) + 1, st = nv % kStages;
             ok = __all_sync(0xffffffffu, mbar_wait(&bar->kv_full[st], (nv / kStages) & 1, abort_word, 0x820));
             if (!ok) break;
@@ -610,30 +601,30 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           uint32_t pk[16], none[16] = {};
           weights_of(pk, 0);
 #pragma unroll
-          for (int other = 1; other < 4; ++other) tmem_st_x16(s_col + ((quad + other) & 3) * 16, none);
-          tmem_st_x16(s_col + quad * 16, pk);
+          for (int other = 1; other < 4; ++other) {
+            const int of = (quad + other) & 3;
+            tmem_st_x16(s_col + (of >> 1) * kHalfKeys + (of & 1) * 16, none);
+          }
+          tmem_st_x16(s_col + (quad >> 1) * kHalfKeys + (quad & 1) * 16, pk);
           tmem_wait_st();
           tc_fence_before_sync();
-          mbar_arrive_warp(&bar->p_part[buf][0], lane);
-          mbar_arrive_warp(&bar->p_part[buf][1], lane);
+          mbar_arrive_warp(&bar->p_full[buf][0], lane);
+          mbar_arrive_warp(&bar->p_full[buf][1], lane);
         } else {
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-#pragma unroll
-            for (int chunk = part == 0 ? 0 : kSplit / 32; chunk < (part == 0 ? kSplit : kKeys) / 32; ++chunk) {
-              uint32_t pk[16];
-              weights_of(pk, chunk * 16);
-              tmem_st_x16(s_col + chunk * 16, pk);
-            }
-            tmem_wait_st();
-            tc_fence_before_sync();
-            mbar_arrive_warp(&bar->p_part[buf][part], lane);
+          for (int chunk = 0; chunk < 2; ++chunk) {
+            uint32_t pk[16];
+            weights_of(pk, chunk * 16);
+            tmem_st_x16(s_col + part0 + chunk * 16, pk);
           }
+          tmem_wait_st();
+          tc_fence_before_sync();
+          mbar_arrive_warp(&bar->p_full[buf][h], lane);
         }
         float s0, s1;
         unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
         l += s0 + s1;
-        ++n;
+       }
       }
       if (!ok) break;
 
