@@ -528,6 +528,23 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           for (int i = 0; i < kMine; ++i)
             if (i < low - k0) sv[i] = __float_as_uint(-INFINITY);
         }
+        // The weights against the reference so far, and the maximum beside them: it is seldom that it has to move, and they are taken again.
+        uint32_t pk[kMine / 2];
+        uint64_t sum2[2];
+        auto weigh = [&]() {
+          const float mc = kBiasProduct ? fmaf(-base, c, ref.offset(c)) : ref.offset(c);
+          const uint64_t c2 = pack_f32x2(c, c), nmc2 = pack_f32x2(-mc, -mc);
+          sum2[0] = sum2[1] = 0;
+#pragma unroll
+          for (int i = 0; i < kMine / 2; ++i) {
+            const uint64_t weights = softmax_weights(sv[2 * i], sv[2 * i + 1], c2, nmc2, weights_on_fma(i));
+            sum2[i & 1] = add_f32x2(sum2[i & 1], weights);
+            float p0, p1;
+            unpack_f32x2(weights, p0, p1);
+            pk[i] = pack2<BF16>(p0, p1);
+          }
+        };
+        weigh();
         float mx[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) mx[u] = __uint_as_float(sv[u]);
@@ -568,6 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
             base = 0.f;
           }
           ref.subtract(sv);
+          weigh();
         }
         if constexpr (PAGED) {
           // the slots behind a sequence's end hold anything: their values become zeros, which their weights, zeros too, need
@@ -582,45 +600,23 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
             fence_proxy_async_smem();
           }
         }
-        const float mc = kBiasProduct ? fmaf(-base, c, ref.offset(c)) : ref.offset(c);
-        const uint64_t c2 = pack_f32x2(c, c), nmc2 = pack_f32x2(-mc, -mc);
-        uint64_t sum2[2] = {0, 0};
-        auto weights_of = [&](uint32_t (&pk)[16], int pair0) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int pair = pair0 + i;
-            const uint64_t weights = softmax_weights(sv[2 * pair], sv[2 * pair + 1], c2, nmc2, weights_on_fma(pair));
-            sum2[i & 1] = add_f32x2(sum2[i & 1], weights);
-            float p0, p1;
-            unpack_f32x2(weights, p0, p1);
-            pk[i] = pack2<BF16>(p0, p1);
-          }
-        };
         if constexpr (SPLIT) {
           // the keys of the other warps have no weight in this warp's copy of the rows
-          uint32_t pk[16], none[16] = {};
-          weights_of(pk, 0);
+          uint32_t none[16] = {};
 #pragma unroll
           for (int other = 1; other < 4; ++other) {
             const int of = (quad + other) & 3;
             tmem_st_x16(s_col + (of >> 1) * kHalfKeys + (of & 1) * 16, none);
           }
           tmem_st_x16(s_col + (quad >> 1) * kHalfKeys + (quad & 1) * 16, pk);
-          tmem_wait_st();
-          tc_fence_before_sync();
-          mbar_arrive_warp(&bar->p_full[buf][0], lane);
-          mbar_arrive_warp(&bar->p_full[buf][1], lane);
         } else {
-#pragma unroll
-          for (int chunk = 0; chunk < 2; ++chunk) {
-            uint32_t pk[16];
-            weights_of(pk, chunk * 16);
-            tmem_st_x16(s_col + part0 + chunk * 16, pk);
-          }
-          tmem_wait_st();
-          tc_fence_before_sync();
-          mbar_arrive_warp(&bar->p_full[buf][h], lane);
+          tmem_st_x16(s_col + part0, *reinterpret_cast<uint32_t(*)[16]>(&pk[0]));
+          tmem_st_x16(s_col + part0 + 16, *reinterpret_cast<uint32_t(*)[16]>(&pk[16]));
         }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive_warp(&bar->p_full[buf][h], lane);
+        if constexpr (SPLIT) mbar_arrive_warp(&bar->p_full[buf][1], lane);
         float s0, s1;
         unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
         l += s0 + s1;
