@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         uint32_t pk[kMine / 2];
         uint64_t sum2[2];
         auto weigh = [&]() {
-          const float mc = kBiasProduct ? fmaf(-base, c, ref.offset(c)) : ref.offset(c);
+          // (a reference far from 0 for the distance alone is near the row's scores in sv: the difference first)
+          const float mc = kBiasProduct && !ref.large ? (ref.m - base) * c : ref.offset(c);
           const uint64_t c2 = pack_f32x2(c, c), nmc2 = pack_f32x2(-mc, -mc);
           sum2[0] = sum2[1] = 0;
 #pragma unroll
@@ -561,6 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         const bool need = ref.asks(m_new, c, kRescaleThreshold) && m_new != -INFINITY;
         if (__any_sync(0xffffffffu, need)) {
           const float f = ref.move(m_new, c);
+          if constexpr (kBiasProduct) ref.large = !(fabsf((m_new - base) * c) <= kFusedReference);
           if (step != first || h > 0) {
             // one P V at most is under way, the last half's: the one before was issued ahead of these scores
             if constexpr (!SPLIT) {
