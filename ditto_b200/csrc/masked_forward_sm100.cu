@@ -34,7 +34,6 @@ constexpr uint32_t kTmemCols = 512, kColO = 256;
 constexpr float kRescaleThreshold = 8.0f;     // log2 units by which a row's maximum may run ahead of its reference
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kSegs = 4;                      // items that the producer is ahead of the others
-constexpr int kHalfKeys = kKeys / 2;
 
 // SPLIT: items of a single token, whose heads (32 at most) fill a part of a tile only.  Four copies of the rows, at rows 0, 32, 64 and 96: a warp has
 // a quarter of a block's keys of each row instead of a thread a whole row, and no weight on the others; the copies' results are summed at an item's
@@ -157,6 +156,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
   static_assert(!SPLIT || (NT == 1 && PAGED), "four copies of an item's rows: single tokens");
   constexpr int kStages = LO::kStages, kAtoms = LO::kAtoms, kTile = LO::kTile;
   constexpr bool kBiasProduct = BIASED && !CAPPED;
+  // a block's scores and weights come in halves, the next one's scores under the other's weights; single tokens' wait for memory, not for these
+  constexpr int kPieces = SPLIT ? 1 : 2, kPiece = kKeys / kPieces;
   // Biased scores grow along a row, by 184 slope a block in units of the exponent: taken from the last block to the first, hardly a row has
   // to move its reference, and its accumulator with it, more than once.
   constexpr bool kBack = kBiasProduct;
@@ -319,12 +320,12 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     // ------------------------------------------------------------ MMA issuer of a buffer (converged warp, elected lane issues)
     const int buf = warp - kMmaWarp, t = NT == 2 ? buf : 0;
     const uint32_t issuer = elect_one();
-    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kHalfKeys, false, false);
+    const uint32_t idesc_s = umma_idesc_f16(BF16, kRows, kPiece, false, false);
     const uint32_t idesc_o = umma_idesc_f16(BF16, kRows, D, false, true);
     const uint64_t dq = umma_desc_sw128(smem_u32(smem + t * kTile), 16, 1024);
     const uint64_t dk0 = umma_desc_sw128(smem_u32(smem + LO::kOffKV), 16, 1024);
     const uint64_t dv0 = umma_desc_sw128(smem_u32(smem + LO::kOffKV), kKeys * 128, 1024);
-    [[maybe_unused]] const uint32_t idesc_bias = umma_idesc_f16(true, kRows, kHalfKeys, false, false);
+    [[maybe_unused]] const uint32_t idesc_bias = umma_idesc_f16(true, kRows, kPiece, false, false);
     [[maybe_unused]] const uint64_t dbias = umma_desc_sw128(smem_u32(smem + LO::kOffBias), 16, 1024);
     const uint32_t d_o = tmem_base + kColO + buf * D, d_s = tmem_base + buf * kKeys;
     auto wait = [&](uint64_t* b, uint32_t parity, uint32_t code) {
@@ -341,16 +342,16 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     auto wait_kv = [&](int n) { return wait(&bar->kv_full[n % kStages], (n / kStages) & 1, 0x310); };      // n: 2 block, or 2 block + 1
     auto issue_s = [&](int block, int h) {
       const int st = (2 * block) % kStages;
-      const uint64_t db = dk0 + ((st * kTile + h * (kHalfKeys * 128)) >> 4);
-      const uint32_t d = d_s + h * kHalfKeys;
+      const uint64_t db = dk0 + ((st * kTile + h * (kPiece * 128)) >> 4);
+      const uint32_t d = d_s + h * kPiece;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const uint32_t off = ((i / 4) * (kRows * 128) + (i % 4) * 32) >> 4;
         umma_ss_elected(d, dq + off, db + off, idesc_s, i > 0 ? 1u : 0u, issuer);
       }
-      if constexpr (kBiasProduct) umma_ss_elected(d, dbias + 2 * t, dbias + 4 + ((h * (kHalfKeys * 128)) >> 4), idesc_bias, 1u, issuer);
+      if constexpr (kBiasProduct) umma_ss_elected(d, dbias + 2 * t, dbias + 4 + ((h * (kPiece * 128)) >> 4), idesc_bias, 1u, issuer);
       umma_commit_elected(&bar->s_full[buf][h], issuer);
-      if (h == 1) umma_commit_elected(&bar->kv_empty[st], issuer);
+      if (h == kPieces - 1) umma_commit_elected(&bar->kv_empty[st], issuer);
     };
     constexpr int kStep = NT == 2 ? 1 : 2;
     uint32_t loads_q = 0, uses_o = 0, n = 0;           // tiles and accumulators so far, steps so far
@@ -384,8 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       if (first < last) {
         ok = wait_kv(2 * (block0 + first));
         if (!ok) break;
-        issue_s(block0 + first, 0);
-        issue_s(block0 + first, 1);
+        for (int h = 0; h < kPieces; ++h) issue_s(block0 + first, h);
       }
       mbar_arrive_warp(&bar->seg_empty[slot], lane);
       if (first + kStep >= last) {                     // Q has been read with the item's last scores
@@ -409,22 +409,24 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         const uint64_t db = dv0 + ((sv * kTile) >> 4);
         auto issue_pv = [&](int h) {
 #pragma unroll
-          for (int i = 0; i < kHalfKeys / 16; ++i)
-            umma_ts_elected(d_o, d_s + h * kHalfKeys + i * 8, db + (((h * (kHalfKeys / 16) + i) * 2048) >> 4), idesc_o, i > 0 || h > 0 || j > first ? 1u : 0u, issuer);
+          for (int i = 0; i < kPiece / 16; ++i)
+            umma_ts_elected(d_o, d_s + h * kPiece + i * 8, db + (((h * (kPiece / 16) + i) * 2048) >> 4), idesc_o, i > 0 || h > 0 || j > first ? 1u : 0u, issuer);
           umma_commit_elected(&bar->pv_done[buf], issuer);
         };
         if (!(ok = wait(&bar->p_full[buf][0], n & 1, 0x340))) break;
         issue_pv(0);
         if (NT == 2 && next < last) issue_s(block0 + next, 0);
-        if (!(ok = wait(&bar->p_full[buf][1], n & 1, 0x341))) break;
-        issue_pv(1);
+        if constexpr (kPieces == 2) {
+          if (!(ok = wait(&bar->p_full[buf][1], n & 1, 0x341))) break;
+          issue_pv(1);
+        }
         umma_commit_elected(&bar->kv_empty[sv], issuer);
         if (next < last) {
           if (NT == 1) {
             if (!(ok = wait_kv(2 * (block0 + next)))) break;
             issue_s(block0 + next, 0);
           }
-          issue_s(block0 + next, 1);
+          if (kPieces == 2) issue_s(block0 + next, 1);
           if (next + kStep >= last) umma_commit_elected(&bar->q_empty[t], issuer);
         } else {
           umma_commit_elected(&bar->o_done[buf], issuer);
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
     float2* sums = reinterpret_cast<float2*>(smem + LO::kOffSum) + row;
     const int in_copy = SPLIT ? lane : row, r_token = in_copy / p.group, r_head = in_copy - r_token * p.group;
     // this thread's keys of a block
-    constexpr int kMine = SPLIT ? 32 : kHalfKeys, kParts = SPLIT ? 1 : 2;
+    constexpr int kMine = SPLIT ? 32 : kPiece;
     const bool row_used = r_token < p.tile_tokens;
     const float c = p.c;
     const int t = NT == 2 ? buf : 0;
@@ -487,11 +489,9 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       const int first = s.template first_step<kBack>(t) + (NT == 1 ? buf : 0), end = s.template last_step<kBack>(t);
       for (int step = first; ok && step < end; step += NT == 1 ? 2 : 1, ++n) {
 #pragma unroll 1
-       for (int h = 0; h < kParts; ++h) {
-        const int part0 = SPLIT ? quad * 32 : h * kHalfKeys;       // this thread's keys of the block begin there
-        ok = SPLIT ? mbar_wait(&bar->s_full[buf][0], n & 1, abort_word, 0x800) && mbar_wait(&bar->s_full[buf][1], n & 1, abort_word, 0x801)
-                   : mbar_wait(&bar->s_full[buf][h], n & 1, abort_word, 0x800);
-        ok = __all_sync(0xffffffffu, ok);
+       for (int h = 0; h < kPieces; ++h) {
+        const int part0 = SPLIT ? quad * 32 : h * kPiece;       // this thread's keys of the block begin there
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[buf][h], n & 1, abort_word, 0x800));
         if (!ok) break;
         tc_fence_after_sync();
         const int j = s.template block<kBack>(step), k0 = j * kKeys + part0;
@@ -528,7 +528,9 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           for (int i = 0; i < kMine; ++i)
             if (i < low - k0) sv[i] = __float_as_uint(-INFINITY);
         }
-        // The weights against the reference so far, and the maximum beside them: it is seldom that it has to move, and they are taken again.
+        // Two tiles, items of many blocks: the weights against the reference so far, and the maximum beside them; it is seldom that it has to move,
+        // and they are taken again.  (16 heads of 64, 8192 x 8192: 486 us instead of 507.)
+        constexpr bool kAhead = NT == 2;
         uint32_t pk[kMine / 2];
         uint64_t sum2[2];
         auto weigh = [&]() {
@@ -545,7 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
             pk[i] = pack2<BF16>(p0, p1);
           }
         };
-        weigh();
+        const bool fresh = step == first && h == 0;    // (no reference yet)
+        if constexpr (kAhead) weigh();
         float mx[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) mx[u] = __uint_as_float(sv[u]);
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         if (__any_sync(0xffffffffu, need)) {
           const float f = ref.move(m_new, c);
           if constexpr (kBiasProduct) ref.large = !(fabsf((m_new - base) * c) <= kFusedReference);
-          if (step != first || h > 0) {
+          if (!fresh) {
             // one P V at most is under way, the last half's: the one before was issued ahead of these scores
             if constexpr (!SPLIT) {
               ok = __all_sync(0xffffffffu, mbar_wait(&bar->pv_done[buf], h ^ 1, abort_word, 0x810));
@@ -587,8 +590,9 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
             base = 0.f;
           }
           ref.subtract(sv);
-          weigh();
+          if constexpr (kAhead) weigh();
         }
+        if constexpr (!kAhead) weigh();
         if constexpr (PAGED) {
           // the slots behind a sequence's end hold anything: their values become zeros, which their weights, zeros too, need
           if (h == 0 && (j + 1) * kKeys > s.keys) {      // (with two tiles both do this, and write the same)
@@ -606,11 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
           // the keys of the other warps have no weight in this warp's copy of the rows
           uint32_t none[16] = {};
 #pragma unroll
-          for (int other = 1; other < 4; ++other) {
-            const int of = (quad + other) & 3;
-            tmem_st_x16(s_col + (of >> 1) * kHalfKeys + (of & 1) * 16, none);
-          }
-          tmem_st_x16(s_col + (quad >> 1) * kHalfKeys + (quad & 1) * 16, pk);
+          for (int other = 1; other < 4; ++other) tmem_st_x16(s_col + ((quad + other) & 3) * 16, none);
+          tmem_st_x16(s_col + quad * 16, pk);
         } else {
           tmem_st_x16(s_col + part0, *reinterpret_cast<uint32_t(*)[16]>(&pk[0]));
           tmem_st_x16(s_col + part0 + 16, *reinterpret_cast<uint32_t(*)[16]>(&pk[16]));
@@ -618,7 +619,6 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         tmem_wait_st();
         tc_fence_before_sync();
         mbar_arrive_warp(&bar->p_full[buf][h], lane);
-        if constexpr (SPLIT) mbar_arrive_warp(&bar->p_full[buf][1], lane);
         float s0, s1;
         unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
         l += s0 + s1;
