@@ -51,12 +51,39 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // ------------------------------------------------------------------ page copies
 constexpr int kCopyThreads = 512, kCopyUnroll = 4;
 
+// What a fork and a compaction do to the tables beside their copies, dealt out over the CTAs of the copy (a launch less each).
+// The child's row of pair i, and one reference more for every page in it: a CTA a pair.
+__device__ __forceinline__ void share_pages(const TableJob& job, const Tables& t, int n) {
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int parent = job.parents[i], child = job.children[i];
+    if (parent < 0 || parent >= t.sequences || child < 0 || child >= t.sequences || parent == child) continue;
+    const long long length = min(static_cast<long long>(max(0, t.lengths[parent])), static_cast<long long>(t.cols) * t.page);
+    const int full = static_cast<int>(length / t.page), last = job.target[i];
+    for (int k = threadIdx.x; k < t.cols; k += blockDim.x) {
+      const int page = k < full ? t.table[parent * t.stride + k] : k == full ? last : -1;
+      t.table[child * t.stride + k] = page;
+      if (page >= 0 && page < t.pages) atomicAdd(t.references + page, 1);
+    }
+    if (threadIdx.x == 0) t.lengths[child] = static_cast<int>(length);
+  }
+}
+__device__ __forceinline__ void rename_pages(const TableJob& job, const Tables& t) {
+  const long long total = static_cast<long long>(t.sequences) * t.cols, step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const long long s = i / t.cols, k = i - s * t.cols;
+    const int page = t.table[s * t.stride + k];
+    job.new_table[s * job.new_stride + k] = page >= 0 && page < t.pages ? job.renamed[page] : page;
+  }
+}
+
 // The pieces of all pages to be copied, in all pools, dealt out evenly: one CTA takes runs of kCopyThreads * kCopyUnroll pieces, each thread
 // with kCopyUnroll loads of 16 bytes in flight.  Bound by the bytes: read once, written once.
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ CopyParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int n = p.n_device != nullptr ? min(*p.n_device, p.n) : p.n;
+  if (p.job.parents != nullptr) share_pages(p.job, p.job.tables, n);
+  if (p.job.renamed != nullptr) rename_pages(p.job, p.job.tables);
   constexpr int kRun = kCopyThreads * kCopyUnroll;
   const int runs = (p.pools.pieces + kRun - 1) / kRun;           // of a page in a pool
   const long long total = static_cast<long long>(n) * p.pools.count * runs;
@@ -239,24 +266,6 @@ __global__ void __launch_bounds__(kTableThreads, 1) fork_pages_kernel(const __gr
     if (target[i] >= 0) target[i] = list[target[i]];
 }
 
-// A CTA a pair: the child's row, and one reference more for every page in it.
-__global__ void __launch_bounds__(256) fork_share_kernel(const __grid_constant__ Tables t, const int* parents, const int* children, const int* target,
-                                                         const int* count) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-  if (*count == 0) return;
-  const int parent = parents[blockIdx.x], child = children[blockIdx.x];
-  if (parent < 0 || parent >= t.sequences || child < 0 || child >= t.sequences || parent == child) return;
-  const long long length = min(static_cast<long long>(max(0, t.lengths[parent])), static_cast<long long>(t.cols) * t.page);
-  const int full = static_cast<int>(length / t.page), last = target[blockIdx.x];
-  for (int k = threadIdx.x; k < t.cols; k += blockDim.x) {
-    const int page = k < full ? t.table[parent * t.stride + k] : k == full ? last : -1;
-    t.table[child * t.stride + k] = page;
-    if (page >= 0 && page < t.pages) atomicAdd(t.references + page, 1);
-  }
-  if (threadIdx.x == 0) t.lengths[child] = static_cast<int>(length);
-}
-
 // One CTA: the k-th live page behind the first n (n live pages) moves to the k-th free place among them.
 __global__ void __launch_bounds__(kTableThreads, 1) compact_pages_kernel(const int* references, int pages, int* new_references, int* renamed, int* source,
                                                                          int* target, int* count) {
@@ -293,17 +302,6 @@ __global__ void __launch_bounds__(kTableThreads, 1) compact_pages_kernel(const i
   }
 }
 
-__global__ void __launch_bounds__(256) rename_kernel(const __grid_constant__ Tables t, int* new_table, long long new_stride, const int* renamed) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const long long total = static_cast<long long>(t.sequences) * t.cols;
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * 256) {
-    const long long s = i / t.cols, k = i - s * t.cols;
-    const int page = t.table[s * t.stride + k];
-    new_table[s * new_stride + k] = page >= 0 && page < t.pages ? renamed[page] : page;
-  }
-}
-
 cudaLaunchConfig_t config(unsigned grid, int threads, cudaStream_t stream, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
@@ -327,7 +325,9 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
 
 cudaError_t launch_copy(const CopyParams& p, int sms, cudaStream_t stream) {
   constexpr int kRun = kCopyThreads * kCopyUnroll;
-  const long long total = static_cast<long long>(p.n) * p.pools.count * ((p.pools.pieces + kRun - 1) / kRun), most = 4ll * sms;
+  const long long copies = static_cast<long long>(p.n) * p.pools.count * ((p.pools.pieces + kRun - 1) / kRun), most = 4ll * sms;
+  const long long entries = p.job.renamed != nullptr ? static_cast<long long>(p.job.tables.sequences) * p.job.tables.cols : 0;
+  const long long renames = (entries + kCopyThreads - 1) / kCopyThreads, total = copies > renames ? copies : renames;
   cudaLaunchAttribute attr[1];
   return launch_kernel(config(static_cast<unsigned>(total < most ? total : most), kCopyThreads, stream, attr), copy_kernel, p);
 }
@@ -345,20 +345,13 @@ cudaError_t launch_reserve(const Tables& t, const int* counts, int* scratch, cud
 cudaError_t launch_fork(const Tables& t, const int* parents, const int* children, int n, int* source, int* target, int* list, int* count,
                         cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
-  const cudaError_t e = launch_kernel(config(1, kTableThreads, stream, attr), fork_pages_kernel, t, parents, children, n, source, target, list, count);
-  if (e != cudaSuccess) return e;
-  return launch_kernel(config(static_cast<unsigned>(n), 256, stream, attr), fork_share_kernel, t, parents, children, target, count);
+  return launch_kernel(config(1, kTableThreads, stream, attr), fork_pages_kernel, t, parents, children, n, source, target, list, count);
 }
 
-cudaError_t launch_compact(const Tables& t, int* new_table, long long new_stride, int* new_references, int* renamed, int* source, int* target,
-                           int* count, cudaStream_t stream) {
+cudaError_t launch_compact(const Tables& t, int* new_references, int* renamed, int* source, int* target, int* count, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
-  const cudaError_t e = launch_kernel(config(1, kTableThreads, stream, attr), compact_pages_kernel, static_cast<const int*>(t.references), t.pages,
-                                      new_references, renamed, source, target, count);
-  if (e != cudaSuccess) return e;
-  const long long ctas = (static_cast<long long>(t.sequences) * t.cols + 255) / 256;
-  return launch_kernel(config(static_cast<unsigned>(ctas < 1024 ? ctas : 1024), 256, stream, attr), rename_kernel, t, new_table, new_stride,
-                       static_cast<const int*>(renamed));
+  return launch_kernel(config(1, kTableThreads, stream, attr), compact_pages_kernel, static_cast<const int*>(t.references), t.pages, new_references,
+                       renamed, source, target, count);
 }
 
 }  // namespace cache

@@ -214,7 +214,8 @@ int check_tables(const ditto_b200_tables* t, bool page_needed, int* status_word,
   return DITTO_OK;
 }
 
-int copy_pages(const ditto_b200_pools* pools, const int* source, const int* target, const int* n_device, int n, int* status_word, cudaStream_t stream) {
+int copy_pages(const ditto_b200_pools* pools, const int* source, const int* target, const int* n_device, int n, const cache::TableJob& job,
+               int* status_word, cudaStream_t stream) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
@@ -227,11 +228,13 @@ int copy_pages(const ditto_b200_pools* pools, const int* source, const int* targ
   p.n = n;
   p.pages = pools->pages;
   p.status = status_word;
+  p.job = job;
   for (int first = 0; first < pools->count; first += cache::kMaxPools) {
     p.pools.count = pools->count - first < cache::kMaxPools ? pools->count - first : cache::kMaxPools;
     for (int i = 0; i < p.pools.count; ++i) p.pools.base[i] = static_cast<uint8_t*>(pools->base[first + i]);
     const cudaError_t e = cache::launch_copy(p, sms, stream);
     if (e != cudaSuccess) return cuda_fail("cache page copy launch", e);
+    p.job = {};                                        // (once)
   }
   return DITTO_OK;
 }
@@ -452,7 +455,7 @@ int ditto_b200_cache_copy(const ditto_b200_pools* pools, const int* source, cons
   const int rc = check_pools(pools);
   if (rc) return rc;
   if (!source || !target || n <= 0) return DITTO_ERR_INVALID_ARG;
-  return copy_pages(pools, source, target, nullptr, n, status_word, static_cast<cudaStream_t>(stream));
+  return copy_pages(pools, source, target, nullptr, n, cache::TableJob{}, status_word, static_cast<cudaStream_t>(stream));
 }
 
 int ditto_b200_cache_free(const ditto_b200_tables* tables, const int* sequences, int n, int* status_word, void* stream) {
@@ -496,7 +499,9 @@ int ditto_b200_cache_fork(const ditto_b200_pools* pools, const ditto_b200_tables
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = cache::launch_fork(t, parents, children, n, source, target, list, count, st);
   if (e != cudaSuccess) return cuda_fail("cache_fork launch", e);
-  return copy_pages(pools, source, target, count, n, status_word, st);
+  cache::TableJob job = {};
+  job.tables = t, job.parents = parents, job.children = children, job.target = target;
+  return copy_pages(pools, source, target, count, n, job, status_word, st);
 }
 
 int ditto_b200_cache_compact(const ditto_b200_pools* pools, const ditto_b200_tables* tables, int* new_table, long long new_stride,
@@ -511,9 +516,11 @@ int ditto_b200_cache_compact(const ditto_b200_pools* pools, const ditto_b200_tab
   int* count = static_cast<int*>(workspace);
   int *source = count + 1, *target = source + t.pages, *renamed = target + t.pages;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = cache::launch_compact(t, new_table, new_stride, new_references, renamed, source, target, count, st);
+  const cudaError_t e = cache::launch_compact(t, new_references, renamed, source, target, count, st);
   if (e != cudaSuccess) return cuda_fail("cache_compact launch", e);
-  return copy_pages(pools, source, target, count, t.pages, status_word, st);
+  cache::TableJob job = {};
+  job.tables = t, job.renamed = renamed, job.new_table = new_table, job.new_stride = new_stride;
+  return copy_pages(pools, source, target, count, t.pages, job, status_word, st);
 }
 
 }  // extern "C"
