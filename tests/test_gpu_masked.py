@@ -72,6 +72,27 @@ def test_modified_scores(cuda, shape, causal, rule):
     _both((q, k, v), g, rules, BF16)
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -40, 2.0 ** -21, 2.0 ** -20, 1.0, 2.0 ** 21], ids=str)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+def test_bias_at_any_scale(cuda, causal, scale):
+    """The bias in units of scores far from 1; three tiles and more keys than queries, so that tiles begin inside a block of keys."""
+    q, k, v, g = _operands(21, 2, 300, 700, 4, 2, 64, BF16)
+    q = (q.float() * (0.125 / scale)).to(BF16)
+    rules = dict(scale=scale, causal=causal, slopes=_slopes(4))
+    out, lse = ops.masked_attention(q, k, v, return_lse=True, **rules)
+    Oracle(q, k, v, **rules).check(out, lse)
+    assert ops.device_status(cuda) == 0
+
+
+def test_bias_of_documents_and_prefixes(cuda):
+    q, k, v, g = _operands(22, 2, 500, 640, 6, 2, 128, BF16)
+    ids = torch.full((2, 640), -1, dtype=torch.int32)
+    ids[0, :300], ids[0, 300:], ids[1, 5:77], ids[1, 77:600] = 4, 9, 1, 2
+    _both((q, k, v), g, dict(scale=128 ** -0.5, causal=True, slopes=_slopes(6), documents=ids.to(cuda)), BF16)
+    prefix = torch.tensor([600, 150], dtype=torch.int32, device=cuda)
+    _both((q, k, v), g, dict(scale=128 ** -0.5, causal=True, slopes=_slopes(6), prefix=prefix), BF16)
+
+
 @pytest.mark.parametrize("prefix", [[0, 0], [1, 400], [129, 128], [-5, 127], [10 ** 9, 300]], ids=str)
 def test_prefix(cuda, prefix):
     q, k, v, g = _operands(6, 2, 300, 400, 4, 2, 64, F16)

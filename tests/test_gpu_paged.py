@@ -101,6 +101,46 @@ def test_chunks(cuda, case, rule):
     c.check(c.attend(**rules), **rules)
 
 
+# lengths, heads, kv heads, d, page: single tokens with rules, shares of the work that end inside a sequence among them
+RULED = [([3000, 1, 129, 64], 8, 2, 128, 32), ([700] * 40, 21, 3, 80, 32), ([5000, 2], 64, 2, 128, 64), ([900, 31], 33, 1, 64, 128),
+         ([9000, 4000, 100], 6, 6, 64, 256)]
+
+
+@pytest.mark.parametrize("rule", ["cap", "slopes", "both", "prefix"])
+@pytest.mark.parametrize("case", RULED, ids=str)
+def test_single_tokens_with_rules(cuda, case, rule):
+    lengths, H, Hk, d, page = case
+    c = Cache(12, lengths, [1] * len(lengths), H, Hk, d, page, BF16)
+    c.append(starts=False)
+    rules = {"scale": d ** -0.5}
+    if rule in ("cap", "both"):
+        rules["cap"] = 4.0
+    if rule in ("slopes", "both"):
+        rules["slopes"] = _slopes(H)
+    if rule == "prefix":
+        rules["prefix"] = torch.tensor([(970 * b) % 3000 for b in range(len(lengths))], dtype=torch.int32, device=cuda)
+    c.check(c.attend(starts=False, **rules), **rules)
+
+
+@pytest.mark.parametrize("new", [1, 40, 700])
+def test_far_keys_and_steep_slopes(cuda, new):
+    """Biases of thousands, in parts of a sequence that hold far keys only; slopes of 0 and below."""
+    c = Cache(13, [9000, 300], [new, 1], 6, 2, 128, 64, F16)
+    c.append()
+    rules = {"scale": 128 ** -0.5, "slopes": torch.tensor([2.0, 0.7, 0.0, 1e-3, 30.0, -1e-3], device=cuda)}
+    c.check(c.attend(**rules), **rules)
+
+
+def test_more_blocks_than_can_be_counted(cuda):
+    """The reach of the table times the heads passes 2^31 blocks: refused, not cut."""
+    pool = torch.zeros(4, 128, 256, 64, dtype=F16, device=cuda)
+    table = torch.zeros(1, 2 ** 23, dtype=torch.int32, device=cuda)
+    query, lengths = torch.zeros(1, 256, 64, dtype=F16, device=cuda), torch.tensor([100], dtype=torch.int32, device=cuda)
+    with pytest.raises((ValueError, RuntimeError)):
+        ops.paged_attention(query, pool, pool, table, lengths)
+    assert (ops.paged_attention(query, pool, pool, table[:, :2 ** 22], lengths) == 0).all()
+
+
 def test_tokens_behind_the_last_sequence_stay(cuda):
     c = Cache(3, [100, 300], [10, 20], 4, 2, 64, 16, F16)
     c.append()
