@@ -1,16 +1,23 @@
 // Gradients of masked attention, from P = 2^(c s - lse):  dV = P^T dO,  dS = P (dO V^T - delta) (1 - tanh^2),  dQ = scale dS K,
 // dK = scale dS^T Q,  delta_i = sum_d dO_id O_id.
 //
-// Three launches: delta with the other things the kernels need of a query row, in tile order; the keys' gradients; the queries'.  The last
-// two compute the scores and dO V^T each for themselves (seven products instead of five), so that every sum stays in tensor memory in one
-// CTA, in a fixed order: no atomics, no accumulator that passes through memory for every block.
+// Four launches: delta with the other things the kernels need of a query row, in tile order; the queries' gradients; the keys'; the sum of
+// what several CTAs have of a block of keys.  The two in the middle compute the scores and dO V^T each for themselves, and the queries' one P K
+// as well (eight products instead of five), so that every sum stays in tensor memory in one CTA, in a fixed order: no atomics, no
+// accumulator that passes through memory for every block, the same bits every time.
 //
+// Sixteen warps of arithmetic, four threads a row with 32 columns each, two MMA warps and a producer.  Tiles come in halves of 64 rows or
+// keys through a ring of four: a half's loads go out as soon as the half two before is done with.
+// Queries: a tile stays, the blocks of keys pass; P and dS go over the scores and dP, the first operands of P K and dS K.  delta is set right
+// from sum_j P (dP - delta), see there.
 // Keys: a block of 128 keys stays, the query tiles pass.  S^T = K Q^T and dP^T = V dO^T have keys as rows, so that P^T and dS^T go back to
-// tensor memory as the first operands of dV += P^T dO and dK += dS^T Q without a transposition.  Two MMA warps: (dV, next S^T) runs under
-// the second half of a tile's arithmetic and (dK, next dP^T) under the first half of the next tile's.  The tiles of all blocks are dealt
-// out in equal shares to the CTAs (causal masks make blocks unequal, shared key heads make them few and long); blocks that a share cuts are
+// tensor memory as the first operands of dV += P^T dO and dK += dS^T Q without a transposition.  The tiles of all blocks are dealt out in
+// equal shares to the CTAs (causal masks make blocks unequal, shared key heads make them few and long); blocks that a share cuts are
 // summed from fp32 parts, in order.
-// Queries: a tile stays, the blocks of keys pass; dS goes over dP, of which there are two so that the next one is ready early.
+//
+// What bounds it: the tensor pipe, at eight products, beside the arithmetic.  16 heads, 8192 x 8192, bf16: d = 128 full 1674 us (821 TFLOP/s
+// counted at five products, 1310 at eight), causal 957 us; d = 64 causal 804 us (the products' shapes are half as deep, the arithmetic is the
+// same).  Of 935 us with a bias by distance, fp16: rows 28, queries 380, keys 487, sums 11 us.
 //
 // fp16: P is taken times 2^14 and dS times a power of two from the largest row norms of dO and V, so that neither leaves the type's range
 // nor falls below its normal numbers as weights of a few thousand keys would.
@@ -73,7 +80,8 @@ __device__ __forceinline__ void dot8(uint4 a, uint4 b, float& dot, float& norm_a
   }
 }
 
-// A CTA half a tile at a time, LANES threads a row of it and kRowsAtOnce rows in flight a thread.  Bound by reading out and its gradient once.
+// A CTA half a tile at a time, LANES threads a row of it and kRowsAtOnce rows in flight a thread.  Bound by reading out and its gradient once:
+// 67 MB of them in 28 us (16 heads of 128, 8192 tokens), most of it latency.
 template <bool BF16, int LANES>
 __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid_constant__ BackwardParams p) {
   grid_dependency_wait();
@@ -657,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) backward_keys_kernel(const __grid
 namespace {
 
 // Sums of the parts of a block that several CTAs had, in the order of its tiles.  CTAs (x, ..) for the block that CTA x of the kernel above
-// began, kSumSlices of them with 1 / kSumSlices of its values each.
+// began, kSumSlices of them with 1 / kSumSlices of its values each.  Bound by reading the parts: 11 us for 148 CTAs' with heads of 128.
 constexpr int kSumThreads = 256, kSumSlices = 8;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kSumThreads) sum_key_parts_kernel(const __grid_constant__ BackwardParams p) {

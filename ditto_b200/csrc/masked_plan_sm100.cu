@@ -45,7 +45,8 @@ __device__ __forceinline__ int block_max(int v, int none, int* scratch, int* bef
 }
 
 // One CTA a batch row.  Document ids may come in any order: a block is skipped where the ranges of ids of its keys and of a tile's queries
-// do not meet, which for documents that follow one another are the blocks that hold none of the tile's, and never one that does.
+// do not meet, which for documents that follow one another are the blocks that hold none of the tile's, and never one that does.  Bound by the
+// latency of its scans and of the reads between them: 13 us for four rows of 4096.
 __global__ void __launch_bounds__(kPlanThreads, 1) document_plan_kernel(const int* documents, const int* prefix, int M, int L, int causal,
                                                                         int tile_tokens, int tiles, int2* runs, int* mixed,
                                                                         KeyBlock* key_blocks, int2* hulls, int2* key_hulls) {
@@ -163,7 +164,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) document_plan_kernel(const in
 }
 
 // Sum of an item's parts, in the order of its keys: O = sum_p 2^(c (m_p - m)) O_p / sum_p 2^(c (m_p - m)) l_p.  CTAs (x, ..) for the item that
-// CTA x of the forward kernel began, a warp a row.
+// CTA x of the forward kernel began, a warp a row.  Bound by reading the parts, which are in L2: 22 us for a chunk of 8192 tokens of 16 heads
+// (37 MB), 5 us for 64 single tokens.
 constexpr int kSumThreads = 256, kSumSlices = 8;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kSumThreads) sum_parts_kernel(const __grid_constant__ Params p, const int rows) {
