@@ -17,7 +17,7 @@
 //
 // What bounds it: the tensor pipe, at eight products, beside the arithmetic.  16 heads, 8192 x 8192, bf16: d = 128 full 1674 us (821 TFLOP/s
 // counted at five products, 1310 at eight), causal 957 us; d = 64 causal 804 us (the products' shapes are half as deep, the arithmetic is the
-// same).  Of 935 us with a bias by distance, fp16: rows 28, queries 380, keys 487, sums 11 us.
+// same).  Of 935 us with a bias by distance, fp16: rows 26, queries 380, keys 487, sums 11 us.
 //
 // fp16: P is taken times 2^14 and dS times a power of two from the largest row norms of dO and V, so that neither leaves the type's range
 // nor falls below its normal numbers as weights of a few thousand keys would.
@@ -67,7 +67,7 @@ __device__ __forceinline__ void ds_scale(const BackwardParams& p, float* up, flo
 }
 
 // ------------------------------------------------------------------ rows
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 
 template <bool BF16>
 __device__ __forceinline__ void dot8(uint4 a, uint4 b, float& dot, float& norm_a) {
@@ -81,7 +81,7 @@ __device__ __forceinline__ void dot8(uint4 a, uint4 b, float& dot, float& norm_a
 }
 
 // A CTA half a tile at a time, LANES threads a row of it and kRowsAtOnce rows in flight a thread.  Bound by reading out and its gradient once:
-// 67 MB of them in 28 us (16 heads of 128, 8192 tokens), most of it latency.
+// 67 MB of them in 26 us (16 heads of 128, 8192 tokens, fp16, with the values for their norms), 34 MB in 12 us (2 x 2047, bf16).
 template <bool BF16, int LANES>
 __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid_constant__ BackwardParams p) {
   grid_dependency_wait();
@@ -94,7 +94,8 @@ __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid
     const int g = at & 1, tile = at / 2 % p.tiles, kv_head = at / 2 / p.tiles % p.kv_heads, b = at / 2 / p.tiles / p.kv_heads;
     const int token0 = tile * p.tile_tokens + g * p.half_tokens;
     uint4 vg[kRowsAtOnce], vo[kRowsAtOnce];
-    int token[kRowsAtOnce], head[kRowsAtOnce];
+    int token[kRowsAtOnce], head[kRowsAtOnce], doc[kRowsAtOnce];
+    float lse[kRowsAtOnce], slope[kRowsAtOnce];
     bool valid[kRowsAtOnce];
 #pragma unroll
     for (int i = 0; i < kRowsAtOnce; ++i) {
@@ -103,6 +104,12 @@ __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid
       head[i] = kv_head * p.group + in_group;
       valid[i] = r < p.half_rows && in_group < p.group && token[i] < p.M;
       vg[i] = vo[i] = make_uint4(0, 0, 0, 0);
+      lse[i] = -INFINITY, doc[i] = -1, slope[i] = 0.f;
+      if (valid[i] && lane == 0) {                     // (all loads of a round go out together)
+        lse[i] = p.lse[(static_cast<size_t>(b) * p.M + token[i]) * p.heads + head[i]];
+        if (p.documents != nullptr) doc[i] = p.documents[static_cast<size_t>(b) * p.L + token[i] + p.L - p.M];
+        if (p.slopes != nullptr) slope[i] = p.slopes[head[i]] * -1.4426950408889634f;
+      }
       if (valid[i] && lane < pieces) {
         vg[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.grad) + 2 * (b * p.g_stride[0] + token[i] * p.g_stride[1] + head[i] * p.g_stride[2]) + lane * 16);
         vo[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.o) + 2 * (b * p.o_stride[0] + token[i] * p.o_stride[1] + head[i] * p.o_stride[2]) + lane * 16);
@@ -121,11 +128,10 @@ __global__ void __launch_bounds__(kRowThreads) backward_rows_kernel(const __grid
       norm_g = fmaxf(norm_g, norm);
       if (lane == 0) {
         const int r = first + i * kSpan, pos = token[i] + p.L - p.M;
-        const float lse = valid[i] ? p.lse[(static_cast<size_t>(b) * p.M + token[i]) * p.heads + head[i]] : -INFINITY;
-        t.lse[r] = lse == -INFINITY ? -INFINITY : fmaf(lse, -1.4426950408889634f, BF16 ? 0.f : kPScaleLog2);
+        t.lse[r] = lse[i] == -INFINITY ? -INFINITY : fmaf(lse[i], -1.4426950408889634f, BF16 ? 0.f : kPScaleLog2);
         t.delta[r] = -dot;
-        t.doc[r] = p.documents != nullptr && valid[i] ? p.documents[static_cast<size_t>(b) * p.L + pos] : -1;
-        t.slope[r] = p.slopes != nullptr && valid[i] ? p.slopes[head[i]] * -1.4426950408889634f : 0.f;
+        t.doc[r] = doc[i];
+        t.slope[r] = slope[i];
         t.pos[r] = static_cast<float>(pos);
       }
     }
@@ -1028,7 +1034,7 @@ cudaError_t launch_backward(const BackwardParams& p, int sms, cudaStream_t strea
     if (e != cudaSuccess) return e;
   }
   cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t rows = config(2 * p.items < 8 * sms ? 2 * p.items : 8 * sms, kRowThreads, 0, stream, attr);
+  const cudaLaunchConfig_t rows = config(2 * p.items < 16 * sms ? 2 * p.items : 16 * sms, kRowThreads, 0, stream, attr);
   const cudaError_t e = D == 64 ? launch_kernel(rows, backward_rows_kernel<BF16, 8>, p) : launch_kernel(rows, backward_rows_kernel<BF16, 16>, p);
   if (e != cudaSuccess) return e;
   if (p.cap_out != 0.f) return launch_products<D, BF16, true, true>(p, sms, stream);      // (with slopes or without)
