@@ -161,7 +161,7 @@ int fill_masked(masked::Params& p, const ditto_b200_masked_args* a) {
 
 // The CTAs of a paged call and the query tiles of its items.
 struct PagedPlan {
-  int grid, tiles, lanes;
+  int grid, tiles, lanes, whole;
   size_t part_ml, parts, bytes;
 };
 int paged_plan(const ditto_b200_paged_args* a, PagedPlan* plan) {
@@ -180,6 +180,12 @@ int paged_plan(const ditto_b200_paged_args* a, PagedPlan* plan) {
   // 425 us instead of 537, of 128: 363 instead of 365; four lanes 443 and 359, eight 450 and 364.
   plan->lanes = a->kv_heads % 2 == 0 && most > sms ? 2 : 1;
   plan->grid = static_cast<int>(most < sms ? most : sms / plan->lanes * plan->lanes);
+  // Single tokens of short sequences: items whole, and so no parts to be summed (a launch less) and no shares to be found.  8 heads over 2 of 64, by the
+  // table's reach of 2, 4, 8 and 16 blocks: one sequence 7.6, 9.8, 14.4 and 23.4 us instead of 11.8, 12.1, 13.7 and 16.1, 32 sequences 8.3, 10.5, 15.1 and 24.0
+  // instead of 12.4, 16.0, 17.8 and 19.4, 200 sequences 16.8, 23.7, 38.5 and 64.6 instead of 26.9, 31.7, 38.4 and 53.2.
+  constexpr long long kWholeBlocks = 6;
+  plan->whole = plan->tiles == 0 && (static_cast<long long>(a->table_cols) * a->page + 127) / 128 <= kWholeBlocks;
+  if (plan->whole) plan->grid = static_cast<int>(items < sms ? items : sms);
   const size_t rows = static_cast<size_t>(plan->grid) * 2 * (plan->tiles == 0 ? 32 : plan->tiles * 128);
   plan->part_ml = up256(rows * d * sizeof(float));
   plan->parts = plan->part_ml + up256(rows * sizeof(float2));
@@ -396,6 +402,7 @@ int ditto_b200_paged_attention(const ditto_b200_paged_args* a, void* workspace, 
   p.page = a->page;
   p.pages = a->pages;
   p.lanes = plan.lanes;
+  p.whole = plan.whole;
   p.status = status_word;
   const long long q_all = a->q_strides[0] * static_cast<long long>(a->tokens);
   rc = map_4d(&p.map_q, bf16, a->q, p.d, p.heads, p.M, 1, a->q_strides[1], a->q_strides[0], q_all, p.group, p.tile_tokens);
@@ -411,7 +418,7 @@ int ditto_b200_paged_attention(const ditto_b200_paged_args* a, void* workspace, 
   p.parts = reinterpret_cast<masked::PartDesc*>(base + plan.parts);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = masked::launch_forward_any(p, d, bf16, true, plan.tiles, plan.grid, st);
-  if (e == cudaSuccess) e = masked::launch_sum_parts(p, d, bf16, plan.tiles, plan.grid, st);
+  if (e == cudaSuccess && !plan.whole) e = masked::launch_sum_parts(p, d, bf16, plan.tiles, plan.grid, st);
   if (e != cudaSuccess) return cuda_fail("paged_attention launch", e);
   return DITTO_OK;
 }

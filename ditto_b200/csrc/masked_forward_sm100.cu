@@ -223,7 +223,14 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
   grid_dependency_wait();
   grid_launch_dependents();
 
-  if constexpr (PAGED) find_start<NT>(p, bar);
+  if constexpr (PAGED) {
+    if (!p.whole) {
+      find_start<NT>(p, bar);
+    } else {
+      if (threadIdx.x == 0) bar->start = {0, 0, 0, 0, 0, 0};
+      __syncthreads();
+    }
+  }
   // The producer finds the items and hands them to the others through shared memory (the registers of the softmax warps are for scores).
   Segment<NT>* segments = reinterpret_cast<Segment<NT>*>(smem + LO::kOffSeg);
   static_assert(sizeof(Segment<NT>) * kSegs <= 512, "segments");

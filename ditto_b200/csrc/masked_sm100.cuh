@@ -57,6 +57,7 @@ struct Params {
   const int* starts;          // [batch + 1], or null: a token a sequence
   long long table_stride;
   int page, pages;
+  int whole;                  // single tokens: CTA x has items x, x + grid, ... whole instead of a share of all blocks
   int lanes;                  // key heads that are worked on side by side: CTA x has heads x % lanes, + lanes, ... of its share of the blocks
   float* part_o;              // [CTA][2][tiles of an item x 128][D]
   float2* part_ml;            // [CTA][2][tiles of an item x 128]: reference (in scores) and sum
@@ -189,6 +190,19 @@ struct PagedWalker {
   Sequence q;
   __device__ __forceinline__ explicit PagedWalker(const PagedStart& s) : at(s), done(0) {}
   __device__ __forceinline__ bool next(const Params& p, Segment<NT>& s) {
+    if (p.whole) {
+      const int item = static_cast<int>(blockIdx.x) + at.left;       // (left counts up by the grid here)
+      if (item >= p.batch * p.kv_heads) return false;
+      at.left += gridDim.x;
+      s.seq = item / p.kv_heads, s.kv_head = item % p.kv_heads;
+      q.load(p, s.seq);
+      s.first_token = 0, s.tokens = q.tokens, s.keys = q.keys, s.row0 = q.row0, s.prefix = q.prefix;
+      s.part = -1, s.at_unit = 0;
+      s.units = q.units<NT>(p, 0);
+      s.clear();
+      s.set(0, 0, (visible_keys(q.keys - 1, q.keys, p.causal, q.prefix) + kKeys - 1) / kKeys);
+      return true;
+    }
     if (at.left <= 0) return false;
     q.load(p, at.seq);
     while (at.first_token >= q.tokens) {        // the next key head, the next sequence with tokens

@@ -141,6 +141,34 @@ def test_more_blocks_than_can_be_counted(cuda):
     assert (ops.paged_attention(query, pool, pool, table[:, :2 ** 22], lengths) == 0).all()
 
 
+@pytest.mark.parametrize("columns", [12, 48, 49], ids=str)
+@pytest.mark.parametrize("sequences", [1, 90, 300])
+def test_short_reach(cuda, sequences, columns):
+    """Tables of a few blocks' reach, on both sides of what is taken whole; more items than CTAs; lengths of 0 and beyond the table."""
+    lengths = [1 + (b * 37) % (16 * columns) for b in range(sequences)]
+    c = Cache(14, lengths, [1] * sequences, 6, 2, 64, 16, F16, columns=columns)
+    c.append(starts=False)
+    rules = {"scale": 0.125, "slopes": _slopes(6)}
+    want = c.attend(starts=False, **rules)
+    c.check(want, **rules)
+    table = c.lengths.clone()
+    c.lengths[0] = 0
+    if sequences > 1:
+        c.lengths[1] = 10 ** 9                          # (ids of -1 among what it reaches)
+    out = c.attend(starts=False, **rules)
+    assert (out[0] == 0).all()
+    ops.device_status(cuda)
+    for b in range(2, sequences):                       # (other lengths cut the work elsewhere, which regroups sums of 32 bits: the bound, not bits)
+        k, v = c.rows[b]
+        Oracle(c.query[None, b:b + 1], k[None], v[None], causal=True, **rules).check(out[None, b:b + 1])
+    c.lengths.copy_(table)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.attend(starts=False, **rules)
+    graph.replay()
+    assert torch.equal(out, want)
+
+
 def test_tokens_behind_the_last_sequence_stay(cuda):
     c = Cache(3, [100, 300], [10, 20], 4, 2, 64, 16, F16)
     c.append()
