@@ -290,17 +290,25 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
         }
         __syncwarp();
       }
+      // lane l's entry of the table for step i, read a step ahead: page l of the block
+      const int page_rows = PAGED ? min(p.page, kKeys) : kKeys;
+      auto pages_of = [&](int j) { return min(kKeys / page_rows, (s.keys - j * kKeys + page_rows - 1) / page_rows); };
+      auto entry = [&](int i) {
+        const int j = s.template block<kBack>(i);
+        return lane < pages_of(j) ? p.table[s.seq * p.table_stride + (j * kKeys + lane * page_rows) / p.page] : -1;
+      };
+      [[maybe_unused]] int ahead = PAGED && s.begin() < s.end() ? entry(s.begin()) : -1;
       for (int i = s.begin(); ok && i < s.end(); ++i) {
         const int j = s.template block<kBack>(i);
         // rows of this block that pages bring: lane i loads page i of the block
-        int page = -1, rows = kKeys, lanes = 1, row_in_page = 0;
+        const int rows = page_rows;
+        int page = -1, lanes = 1, row_in_page = 0;
         if constexpr (PAGED) {
-          rows = min(p.page, kKeys);
-          const int k0 = j * kKeys + lane * rows, per_block = kKeys / rows;
-          lanes = min(per_block, (s.keys - j * kKeys + rows - 1) / rows);
+          lanes = pages_of(j);
           row_in_page = (j * kKeys) % p.page;          // (0 unless a page is longer than a block)
+          page = ahead;
+          if (i + 1 < s.end()) ahead = entry(i + 1);
           if (lane < lanes) {
-            page = p.table[s.seq * p.table_stride + k0 / p.page];
             if (page < 0 || page >= p.pages) {
               page = -1;                               // (out of the map's range: zeros)
               if (p.status != nullptr) atomicCAS(p.status, 0, kBadPage);
