@@ -17,7 +17,7 @@
 //
 // Over a paged cache the blocks of all items are dealt out to the CTAs in equal shares, whatever the sequences' lengths: an item that a
 // share cuts is finished by a second kernel from fp32 parts.  8192 tokens over 16384 keys, 16 heads over two of 128, biased: 809 us for this
-// kernel, 22 us for the second; with single tokens it is bound by its reads (SPLIT, below).
+// kernel, 19 us for the second; with single tokens it is bound by its reads (SPLIT, below).
 #include <atomic>
 
 #include "host_util.cuh"
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_forward_kernel(const __gri
       float l = 0.f;
       const int first = s.template first_step<kBack>(t) + (NT == 1 ? buf : 0), end = s.template last_step<kBack>(t);
       for (int step = first; ok && step < end; step += NT == 1 ? 2 : 1, ++n) {
-#pragma unroll 1
+#pragma unroll 1                                       // (unrolled 6 to 18 % slower: twice the code)
        for (int h = 0; h < kPieces; ++h) {
         const int part0 = SPLIT ? quad * 32 : h * kPiece;       // this thread's keys of the block begin there
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->s_full[buf][h], n & 1, abort_word, 0x800));
