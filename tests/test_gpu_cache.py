@@ -215,6 +215,24 @@ def test_a_serving_run(cuda):
     assert ops.device_status(cuda) == 0
 
 
+def test_more_pools_than_a_launch_takes(cuda):
+    """Fork and compaction of 300 pools: copies in two launches, the tables once."""
+    m = Model(4, 5, 30, 4)
+    t = Tables(m, _pools(300, 30, (4, 4), torch.float32, cuda), cuda)
+    counts = [6, 9, 3, 0]
+    m.reserve(counts)
+    ops.cache_reserve(t.table, t.lengths, t.refs, t.ids(counts), 4)
+    m.fork([1], [3])
+    ops.cache_fork(t.pools, t.table, t.lengths, t.refs, t.ids([1]), t.ids([3]), 4)
+    t.check()
+    m.free([0])
+    ops.cache_free(t.table, t.lengths, t.refs, t.ids([0]))
+    m.compact()
+    t.table, t.refs = ops.cache_compact(t.pools, t.table, t.refs)
+    t.check()
+    assert ops.device_status(cuda) == 0
+
+
 def test_captured_fork(cuda):
     """A fork in a graph follows the tables' contents at each replay."""
     m = Model(6, 5, 40, 4)
