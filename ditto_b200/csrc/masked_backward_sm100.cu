@@ -945,7 +945,9 @@ __global__ void __launch_bounds__(kThreads, 1) backward_queries_kernel(const __g
       if (!ok) break;
       const float off_by = (mine[0] + mine[128] + mine[256] + mine[384]) * (CAPPED ? p_down : down);
       if (part_of_row == 0 && valid) rows.delta[r_in] = delta - off_by;
-      const float scale = p.scale * down, scale_pk = -p.scale * off_by * p_down;
+      // (a row that sees one key: nothing, and not what rounding leaves of it; the keys' dS is 0 by itself, delta being dP)
+      const bool lone = !mixed && limit - low == 1;
+      const float scale = lone ? 0.f : p.scale * down, scale_pk = lone ? 0.f : -p.scale * off_by * p_down;
       uint8_t* dst = static_cast<uint8_t*>(p.dq) + 2 * ((static_cast<size_t>(s.seq) * p.M + token) * p.heads + s.kv_head * p.group + r_head) * p.d;
 #pragma unroll
       for (int cc = 0; cc < D / 4; cc += 16) {

@@ -93,6 +93,27 @@ def test_bias_of_documents_and_prefixes(cuda):
     _both((q, k, v), g, dict(scale=128 ** -0.5, causal=True, slopes=_slopes(6), prefix=prefix), BF16)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("d", [40, 64, 128])
+@pytest.mark.parametrize("rule", ["plain", "cap", "slopes"])
+def test_rows_that_see_one_key(cuda, rule, d, dtype):
+    """Their weight is 1 whatever the score: gradients of queries and keys are exactly 0, that of a value its rows' sum."""
+    rules = dict(scale=d ** -0.5, causal=True)
+    if rule == "cap":
+        rules["cap"] = 30.0
+    if rule == "slopes":
+        rules["slopes"] = _slopes(8)
+    ids = torch.arange(200, dtype=torch.int32, device=cuda).expand(3, 200).contiguous()
+    for M, documents in ((1, None), (200, ids)):
+        q, k, v, g = _operands(23, 3, M, M, 8, 2, d, dtype)
+        out, lse = ops.masked_attention(q, k, v, return_lse=True, documents=documents, **rules)
+        dq, dk, dv = ops.masked_attention_backward(g, q, k, v, out, lse, documents=documents, **rules)
+        assert torch.equal(out, v.repeat_interleave(4, 2)) and (dq == 0).all() and (dk == 0).all()
+        want = g.double().view(3, M, 2, 4, d).sum(3)
+        u = torch.finfo(dtype).eps / 2                  # (rounded once; weights within 2^-20 of 1 are 1 in 16 bits)
+        assert ((dv.double() - want).abs() <= u * want.abs() + 2.0 ** -20 * g.double().abs().amax() * 4).all()
+
+
 @pytest.mark.parametrize("prefix", [[0, 0], [1, 400], [129, 128], [-5, 127], [10 ** 9, 300]], ids=str)
 def test_prefix(cuda, prefix):
     q, k, v, g = _operands(6, 2, 300, 400, 4, 2, 64, F16)
