@@ -158,6 +158,8 @@ def masked_attention(query, key, value, out=None, scale=1.0, causal=False, prefi
     Returns out [batch, M, heads, d] = softmax over what is seen, times value (0 for a row that sees nothing), and with return_lse also the
     float32 log of the sum of exponentials [batch, M, heads] (-inf for such a row; it gets no gradient).  Gradients of query, key and value
     flow where autograd asks for them (`out` cannot be given then).
+    Values that a row does not see have weight 0 and must be finite, padding included; keys that it does not see may be anything here, and must be
+    finite where there are gradients.
     """
     if _ops._fast is not None:
         r = _ops._fast.masked(query, key, value, out, scale, causal, prefix, documents, slopes, cap, return_lse)
